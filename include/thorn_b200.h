@@ -370,6 +370,91 @@ THORN_API int thorn_magma_stats_multi(const thorn_magma_tensor* tensors, int n, 
                                       void* stream);
 
 /* --------------------------------------------------------------------------
+ * Optimizer state in 8 bits and in 32 (no counterpart in the reference, which
+ * keeps state in the parameter dtype and updates 16-bit parameters in place).
+ *
+ * 8-bit state: e4m3 codes, one byte per element, in blocks of 128 consecutive
+ * elements with one scale byte each: value = code * 2^(byte - 127).  The byte is
+ * the smallest with max|x| <= 448 * 2^(byte - 127) (at least 0; 0 for a block of
+ * zeros).  A block that holds a value that is not finite gets byte 255 and reads
+ * back as NaN.  Zeroed codes and scales are a zero state.  Codes are rounded
+ * stochastically: |x| * 2^(127 - byte) rounds up with the probability of its
+ * distance to the lower code, from 16 bits of a counter-based generator keyed by
+ * `seed` (give every tensor and every step its own).  Elements 4q..4q+3 of a run
+ * (a tensor; for thorn_momentum8_multi each matrix) share one 32-bit number.
+ *   key = z3 ^ (z3 >> 32), z1 = seed + 0x9E3779B97F4A7C15,
+ *     z2 = (z1 ^ (z1 >> 32)) * 0x6A09E667F3BCC909, z3 = (z2 ^ (z2 >> 29)) * 0xBB67AE8584CAA73B
+ *   a = lo32(q) * 0x9E3779B9 + lo32(key);  fold(x, y) = hi32(x y) ^ lo32(x y)
+ *   x = fold(a, a ^ hi32(key) ^ (hi32(q) + run));  r = fold(x, x ^ 0xBB67AE85)
+ * elements 4q and 4q+2 read the low and high half of r as a fraction of 2^16,
+ * 4q+1 and 4q+3 read them with their bits in reversed order.
+ *
+ * thorn_adamw8_multi: thorn_adamw_multi's step with both moments in 8 bits; the
+ *   update uses the moments before they are rounded.  In a block whose second
+ *   moments are not all zero each is held at no less than the smallest code.
+ * thorn_adamw_master_multi: fp32 moments and fp32 master weights.
+ * With w set (required by the second, optional for 16-bit parameters in the
+ * first) the update is applied to w and p receives w rounded once.
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  void* p;            /* param (p_dtype); NULL: update the moments only */
+  const void* g;      /* grad (p_dtype) */
+  void* w;            /* fp32 master weights, or NULL */
+  void* m;            /* first moment: e4m3 codes or fp32 */
+  void* v;            /* second moment: e4m3 codes or fp32 */
+  void* m_scale;      /* [ceil(numel / 128)] scale bytes (8-bit state only) */
+  void* v_scale;
+  int64_t numel;
+  uint64_t seed;      /* 8-bit state only */
+  float lr;           /* as in thorn_adam_tensor */
+  float bc1;
+  float bc2;
+  int32_t degenerate;
+} thorn_adamw_state_tensor;
+
+THORN_API int thorn_adamw8_multi(const thorn_adamw_state_tensor* tensors, int n, int p_dtype, double beta1,
+                                 double beta2, float weight_decay, float eps, void* stream);
+THORN_API int thorn_adamw_master_multi(const thorn_adamw_state_tensor* tensors, int n, int p_dtype, double beta1,
+                                       double beta2, float weight_decay, float eps, void* stream);
+
+/* Orthogonalized group with the momentum in 8 bits:  m <- beta1 m + g, rounded
+ * to 8 bits (the blocks restart at each matrix of the batch);  u = g + beta1 m
+ * from the rounded m;  x = u / (||u||_F + 1e-8) per matrix, rounded once to
+ * x_dtype (fp16 or bf16), in rows of leading dimension ldx.  x == NULL: the
+ * momentum only.  Scratch need not be cleared. */
+typedef struct {
+  const void* g;      /* grad (p_dtype), [batch, rows, cols] */
+  void* m;            /* e4m3 codes, same shape */
+  void* m_scale;      /* [batch][ceil(rows * cols / 128)] scale bytes */
+  void* x;            /* out [batch, rows, ldx] or NULL */
+  int64_t batch, rows, cols;
+  int64_t ldx;        /* >= cols */
+  uint64_t seed;
+  void* scratch;      /* with x: thorn_momentum8_scratch_bytes(batch, rows, cols) bytes, 4-byte aligned */
+} thorn_momentum8_tensor;
+
+THORN_API int64_t thorn_momentum8_scratch_bytes(int64_t batch, int64_t rows, int64_t cols);
+THORN_API int thorn_momentum8_multi(const thorn_momentum8_tensor* tensors, int n, int p_dtype, int x_dtype,
+                                    float beta1, void* stream);
+
+/* thorn_ortho_post_multi onto fp32 master weights: u = U * row_scale (* gscale_b
+ * from mat_stats, as thorn_pnn_stats_multi gives it for p_dtype fp32),
+ * u <- u + wd w where u w >= 0, w <- w - lr u, p = w rounded once.  U and p are
+ * 16-bit types; U is used as it is. */
+typedef struct {
+  const void* U;           /* u_dtype [batch, rows, cols] */
+  void* p;                 /* out, p_dtype */
+  float* w;                /* master weights */
+  const float* row_scale;  /* NULL: no row scaling */
+  const float* mat_stats;  /* NULL: row_scale is the final factor */
+  int64_t batch, rows, cols;
+  float lr;
+} thorn_apply_master_tensor;
+
+THORN_API int thorn_apply_master_multi(const thorn_apply_master_tensor* tensors, int n, int u_dtype, int p_dtype,
+                                       float weight_decay, void* stream);
+
+/* --------------------------------------------------------------------------
  * Peer-memory exchange of the FSDP2 Shard(0) path (THORN.exchange = "peer").
  * Replaces the reference's per-matrix dist.gather / dist.scatter of fp32 rows
  * (_DistributedTHORNState.gather / scatter, thorn.py:1023-1122) for ranks of one

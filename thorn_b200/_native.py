@@ -61,6 +61,23 @@ class MagmaTensor(Structure):
                 ("out", c_void_p), ("scratch", c_void_p)]
 
 
+class AdamStateTensor(Structure):
+    _fields_ = [("p", c_void_p), ("g", c_void_p), ("w", c_void_p), ("m", c_void_p), ("v", c_void_p),
+                ("m_scale", c_void_p), ("v_scale", c_void_p), ("numel", c_int64), ("seed", c_uint64),
+                ("lr", c_float), ("bc1", c_float), ("bc2", c_float), ("degenerate", c_int32)]
+
+
+class Momentum8Tensor(Structure):
+    _fields_ = [("g", c_void_p), ("m", c_void_p), ("m_scale", c_void_p), ("x", c_void_p),
+                ("batch", c_int64), ("rows", c_int64), ("cols", c_int64), ("ldx", c_int64), ("seed", c_uint64),
+                ("scratch", c_void_p)]
+
+
+class ApplyMasterTensor(Structure):
+    _fields_ = [("U", c_void_p), ("p", c_void_p), ("w", c_void_p), ("row_scale", c_void_p), ("mat_stats", c_void_p),
+                ("batch", c_int64), ("rows", c_int64), ("cols", c_int64), ("lr", c_float)]
+
+
 class MdPrepTensor(Structure):
     _fields_ = [("gain", c_void_p), ("sp", c_void_p), ("sig", c_void_p), ("n", c_int64)]
 
@@ -123,6 +140,17 @@ _PROTOS = {
     "thorn_peer_wait": (c_int, [c_void_p, c_int, c_uint64, c_uint64, c_void_p, c_void_p]),
 }
 
+# the optimizer-state operators (thorn_b200/multi.py)
+_STATE_PROTOS = {
+    "thorn_adamw8_multi": (c_int, [POINTER(AdamStateTensor), c_int, c_int, c_double, c_double, c_float, c_float,
+                                   c_void_p]),
+    "thorn_adamw_master_multi": (c_int, [POINTER(AdamStateTensor), c_int, c_int, c_double, c_double, c_float, c_float,
+                                         c_void_p]),
+    "thorn_momentum8_scratch_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "thorn_momentum8_multi": (c_int, [POINTER(Momentum8Tensor), c_int, c_int, c_int, c_float, c_void_p]),
+    "thorn_apply_master_multi": (c_int, [POINTER(ApplyMasterTensor), c_int, c_int, c_int, c_float, c_void_p]),
+}
+
 _lock = threading.Lock()
 _lib = None
 
@@ -146,7 +174,7 @@ def load(build_if_missing: bool = False):
                 raise RuntimeError(
                     f"thorn_b200 CUDA library not found at {path}; build it with `python -m thorn_b200.build`")
         lib = ctypes.CDLL(path)
-        for name, (res, args) in _PROTOS.items():
+        for name, (res, args) in {**_PROTOS, **_STATE_PROTOS}.items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
