@@ -11,7 +11,6 @@
 //
 // Every kernel runs over flat chunks of 8192 elements with 8 consecutive elements per
 // thread, so 16 lanes hold one block of 128 and its maximum takes four shuffles.
-#include <cuda_fp8.h>
 #include <math.h>
 
 #include "common.cuh"
@@ -112,8 +111,35 @@ __device__ __forceinline__ uint32_t encode4(float y0, float y1, float y2, float 
   return d;
 }
 
-// 8 codes -> 8 fp32 values of the codes (the block's scale is not applied)
-__device__ __forceinline__ void decode8(uint2 c, float* v) {
+// Two fp32 values in one 64-bit register pair: Blackwell's packed multiply and fma round
+// each half like the scalar instruction and take one issue slot for both.  The 8-bit
+// kernels are bound by instruction issue, not by the fp32 pipes.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pack_f2(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack_f2(f2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ f2 dup(float a) { return pack_f2(a, a); }
+__device__ __forceinline__ f2 mul(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// 8 codes -> the 8 fp32 values of the codes as pairs (the block's scale is not applied)
+__device__ __forceinline__ void decode8(uint2 c, f2* v) {
   const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -121,9 +147,23 @@ __device__ __forceinline__ void decode8(uint2 c, float* v) {
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
         : "=r"(h0), "=r"(h1)
         : "r"(w[i]));
-    unpack2(h0, v[4 * i], v[4 * i + 1], (__half*)nullptr);
-    unpack2(h1, v[4 * i + 2], v[4 * i + 3], (__half*)nullptr);
+    float a, b;
+    unpack2(h0, a, b, (__half*)nullptr);
+    v[2 * i] = pack_f2(a, b);
+    unpack2(h1, a, b, (__half*)nullptr);
+    v[2 * i + 1] = pack_f2(a, b);
   }
+}
+__device__ __forceinline__ uint2 encode8(const f2* y, uint32_t r0, uint32_t r1) {
+  float a, b, c, d;
+  uint2 o;
+  unpack_f2(y[0], a, b);
+  unpack_f2(y[1], c, d);
+  o.x = encode4(a, b, c, d, r0);
+  unpack_f2(y[2], a, b);
+  unpack_f2(y[3], c, d);
+  o.y = encode4(a, b, c, d, r1);
+  return o;
 }
 
 // 2^(b - 127), NaN for b = 255
@@ -136,35 +176,39 @@ __device__ __forceinline__ float scale_inverse(uint32_t b) {
 }
 
 // The upper 16 bits of max|v| of 8 values, rounded up: enough for the block's scale (the
-// only mantissa it is compared with is 1.75), and two of them fit one shuffle.  Integer
-// maxima keep a NaN (its bits are above infinity's).  Magnitudes from 2^128 - 2^120 up
-// round to infinity.
-__device__ __forceinline__ uint32_t top16(const float* v) {
-  uint32_t t = 0;
+// only mantissa it is compared with is 1.75), and two of them fit one shuffle.  A NaN
+// stays one.  Magnitudes from 2^128 - 2^120 up round to infinity.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t top16(const f2* v) {
+  float x[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) t = max(t, __float_as_uint(v[k]) & 0x7fffffffu);
-  return (t + 0xffffu) >> 16;
+  for (int k = 0; k < 4; ++k) unpack_f2(v[k], x[2 * k], x[2 * k + 1]);
+  const float t = max3_abs(max3_abs(x[0], x[1], x[2]), max3_abs(x[3], x[4], x[5]), max3_abs(x[6], x[7], x[7]));
+  return (__float_as_uint(t) + 0xffffu) >> 16;
 }
 
 // Scale byte of a block from its top16: the smallest power of two with max <= 448 * 2^k
 // (448 = 1.75 * 2^8 is the largest e4m3 value); 255 for a block that is not finite.
 __device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
-  if (top >= 0x7f80u) return 255u;
-  const int b = (int)((top + 0x1fu) >> 7) - 8;
-  return b < 0 ? 0u : (uint32_t)b;
+  const int b = max((int)((top + 0x1fu) >> 7) - 8, 0);
+  return top >= 0x7f80u ? 255u : (uint32_t)b;
 }
 
 // ---------------------------------------------------------------------------
-// 8 consecutive elements as they lie in memory
+// 8 consecutive elements as they lie in memory.  FULL: all 8 are inside the tensor and
+// aligned for vector accesses; otherwise the first n, one by one, zeros behind them.
 // ---------------------------------------------------------------------------
 template <class T>
 struct Raw8 {
   uint4 x[sizeof(T) / 2];
 };
-template <class T>
-__device__ __forceinline__ Raw8<T> load_raw(const T* p, int n, bool full) {
-  Raw8<T> r;
-  if (full) {
+template <bool FULL, class T>
+__device__ __forceinline__ void load_raw(const T* p, int n, Raw8<T>& r) {
+  if constexpr (FULL) {
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.x[i] = reinterpret_cast<const uint4*>(p)[i];
   } else {
@@ -173,42 +217,133 @@ __device__ __forceinline__ Raw8<T> load_raw(const T* p, int n, bool full) {
     for (int k = 0; k < 8; ++k) e[k] = k < n ? p[k] : from_f<T>(0.f);
     memcpy(&r, e, sizeof(r));
   }
-  return r;
 }
 template <class T>
-__device__ __forceinline__ void unpack_raw(const Raw8<T>& r, float* v) {
+__device__ __forceinline__ void values(const Raw8<T>& r, f2* v) {
   if constexpr (std::is_same<T, float>::value) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      v[4 * i] = __uint_as_float(r.x[i].x);
-      v[4 * i + 1] = __uint_as_float(r.x[i].y);
-      v[4 * i + 2] = __uint_as_float(r.x[i].z);
-      v[4 * i + 3] = __uint_as_float(r.x[i].w);
-    }
+    memcpy(v, &r, sizeof(r));
   } else {
-    unpack2(r.x[0].x, v[0], v[1], (T*)nullptr);
-    unpack2(r.x[0].y, v[2], v[3], (T*)nullptr);
-    unpack2(r.x[0].z, v[4], v[5], (T*)nullptr);
-    unpack2(r.x[0].w, v[6], v[7], (T*)nullptr);
+    const uint32_t w[4] = {r.x[0].x, r.x[0].y, r.x[0].z, r.x[0].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float a, b;
+      unpack2(w[k], a, b, (T*)nullptr);
+      v[k] = pack_f2(a, b);
+    }
   }
 }
-__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n, bool full) {
-  if (full) return *reinterpret_cast<const uint2*>(p);
+template <bool FULL, class T>
+__device__ __forceinline__ void store8(T* p, const f2* v, int n) {
+  if constexpr (FULL && std::is_same<T, float>::value) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) reinterpret_cast<ulonglong2*>(p)[i] = make_ulonglong2(v[2 * i], v[2 * i + 1]);
+  } else {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) unpack_f2(v[k], x[2 * k], x[2 * k + 1]);
+    store_n(p, x, FULL ? 8 : n, FULL);
+  }
+}
+template <bool FULL>
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n) {
+  if constexpr (FULL) return *reinterpret_cast<const uint2*>(p);
   uint32_t w[2] = {0u, 0u};
 #pragma unroll
   for (int k = 0; k < 8; ++k)
     if (k < n) w[k >> 2] |= (uint32_t)p[k] << (8 * (k & 3));
   return make_uint2(w[0], w[1]);
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, uint2 c, int n, bool full) {
-  if (full) {
+template <bool FULL>
+__device__ __forceinline__ void store_codes(uint8_t* p, uint2 c, int n) {
+  if constexpr (FULL) {
     *reinterpret_cast<uint2*>(p) = c;
-    return;
-  }
-  const uint32_t w[2] = {c.x, c.y};
+  } else {
+    const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k < n) p[k] = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
+    for (int k = 0; k < 8; ++k)
+      if (k < n) p[k] = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
+  }
+}
+
+// A warp's segment of a chunk is kStSeg consecutive elements, taken 256 at a time: 8 blocks
+// of 128, whose 8 scale bytes it reads and writes as one word each.  Bytes written block by
+// block and read a moment later from the same 32-byte sector stalled the momentum pass on
+// 16384 x 4096 at 145 us.  Iteration `it` of the lanes' half `half` uses byte 2 it + half.
+constexpr int kStSeg = kStChunk / (kStThreads / 32);
+constexpr int kStIter = kStSeg / 256;
+static_assert(kStIter == 4 && kStSeg == 8 * kQBlock, "a segment's scale bytes are one 8-byte word");
+
+// This lane's half's bytes of iterations 0..3, the first in the low byte.  A matrix of a
+// stack may start its scales at any byte.
+__device__ __forceinline__ uint32_t load_seg_bytes(const uint8_t* p) {
+  const int half = (threadIdx.x >> 4) & 1;
+  if ((reinterpret_cast<uintptr_t>(p) & 7u) == 0) {
+    const uint2 s = *reinterpret_cast<const uint2*>(p);
+    return __byte_perm(s.x, s.y, half ? 0x7531 : 0x6420);
+  }
+  return p[half] | (uint32_t)p[2 + half] << 8 | (uint32_t)p[4 + half] << 16 | (uint32_t)p[6 + half] << 24;
+}
+__device__ __forceinline__ uint32_t seg_byte(uint32_t b, int it) { return (b >> (8 * it)) & 0xffu; }
+__device__ __forceinline__ void store_seg_bytes(uint8_t* p, uint32_t b) {
+  const uint32_t o = __shfl_xor_sync(0xffffffffu, b, 16);
+  if ((threadIdx.x & 31) == 0) {
+    const uint2 s = make_uint2(__byte_perm(b, o, 0x5140), __byte_perm(b, o, 0x7362));
+    if ((reinterpret_cast<uintptr_t>(p) & 7u) == 0) {
+      *reinterpret_cast<uint2*>(p) = s;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) p[k] = (uint8_t)((k < 4 ? s.x : s.y) >> (8 * (k & 3)));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the update's arithmetic
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float rsqrt_approx(float x) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float sqrt_approx(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// atan2(y, sqrt(x2)) of two elements, x2 >= 0: the angle of t = |y| / sqrt(x2), from t or
+// 1/t in [0, 1].  x2 is taken 2^-126 higher (nothing in fp32 from 2^-102 up), so that zero
+// over zero is zero and a subnormal x2 needs no case of its own; it acts like an eps of
+// 1e-19 beside the root.  The polynomial in s^2 is the minimax fit of atan(s)/s on [0, 1]
+// with eight coefficients (Remez exchange: 9.9e-8 relative, 2.1e-7 with the roundings of
+// its fp32 evaluation).  The general function, with an exact square root and divisions,
+// made the 8-bit step of two 128256 x 4096 tensors 4108 us where this makes it 3103.
+__device__ __forceinline__ f2 angle2(f2 y, f2 x2) {
+  float y0, y1, q0, q1;
+  unpack_f2(y, y0, y1);
+  unpack_f2(add(x2, dup(1.17549435e-38f)), q0, q1);
+  const float t0 = fabsf(y0) * rsqrt_approx(q0), t1 = fabsf(y1) * rsqrt_approx(q1);
+  const bool b0 = t0 > 1.f, b1 = t1 > 1.f;
+  const f2 s = pack_f2(b0 ? rcp_approx(t0) : t0, b1 ? rcp_approx(t1) : t1);
+  const f2 z = mul(s, s);
+  f2 p = dup(-0.0046932776f);
+  p = fma(p, z, dup(0.02425241f));
+  p = fma(p, z, dup(-0.0594864f));
+  p = fma(p, z, dup(0.09914293f));
+  p = fma(p, z, dup(-0.14019482f));
+  p = fma(p, z, dup(0.19969724f));
+  p = fma(p, z, dup(-0.3333199f));
+  p = fma(p, z, dup(0.9999999f));
+  float a0, a1;
+  unpack_f2(mul(s, p), a0, a1);
+  a0 = b0 ? 1.57079632679f - a0 : a0;
+  a1 = b1 ? 1.57079632679f - a1 : a1;
+  return pack_f2(copysignf(a0, y0), copysignf(a1, y1));
 }
 
 // ===========================================================================
@@ -224,12 +359,13 @@ struct StAdam {
   uint8_t* vs;
   int64_t numel;
   uint64_t key;
-  float lr, bc1, bc2;
+  float lr;
+  float c, eps;  // bc1 / sqrt(bc2), eps / sqrt(bc2): u = c m / (sqrt(v) + eps)
   int degenerate;
   int vec;
 };
 struct StAdamScalars {
-  float w1, beta2, w2, wd, eps;  // w1 = 1 - beta1, w2 = 1 - beta2, formed in double
+  float w1, beta2, w2, wd;  // w1 = 1 - beta1, w2 = 1 - beta2, formed in double
 };
 template <int CAP>
 struct StAdamArgs {
@@ -237,90 +373,165 @@ struct StAdamArgs {
   StAdamScalars s;
 };
 
+// What a thread reads for 8 elements.
+template <class P, bool S8, bool MASTER>
+struct AdamIn {
+  using W = std::conditional_t<MASTER, float, P>;
+  using S = std::conditional_t<S8, uint2, Raw8<float>>;
+  Raw8<P> g;
+  Raw8<W> w;
+  S m, v;
+};
+template <bool FULL, class P, bool S8, bool MASTER>
+__device__ __forceinline__ void adam_load(const StAdam& e, int64_t i0, int n, AdamIn<P, S8, MASTER>& in) {
+  using W = typename AdamIn<P, S8, MASTER>::W;
+  load_raw<FULL>((const P*)e.g + i0, n, in.g);
+  if constexpr (S8) {
+    in.m = load_codes<FULL>((const uint8_t*)e.m + i0, n);
+    in.v = load_codes<FULL>((const uint8_t*)e.v + i0, n);
+  } else {
+    load_raw<FULL>((const float*)e.m + i0, n, in.m);
+    load_raw<FULL>((const float*)e.v + i0, n, in.v);
+  }
+  if (e.p != nullptr) load_raw<FULL>((const W*)(MASTER ? (void*)e.w : e.p) + i0, n, in.w);
+}
+
+// One thread's 8 elements at i0; mb, vb: the scale bytes of their block, read and written.
+// The moments are formed with the roundings of separate fp32 operations (the products with
+// the power-of-two scales inside the fmas are exact).
+template <bool FULL, class P, bool S8, bool MASTER>
+__device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars& sc, int64_t i0, int n,
+                                           const AdamIn<P, S8, MASTER>& in, uint32_t& mb, uint32_t& vb) {
+  f2 g[4], m[4], v[4];
+  const f2 w1 = dup(sc.w1), w2 = dup(sc.w2);
+  values(in.g, g);
+  if constexpr (S8) {
+    decode8(in.m, m);
+    decode8(in.v, v);
+    const float ms1 = scale_value(mb);
+    const f2 ms = dup(ms1), neg = dup(-ms1), vs = dup(scale_value(vb) * sc.beta2);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      m[k] = fma(m[k], ms, mul(fma(m[k], neg, g[k]), w1));
+      v[k] = add(mul(v[k], vs), mul(mul(g[k], g[k]), w2));
+    }
+    uint32_t top = top16(m) | (top16(v) << 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+    mb = scale_byte(top & 0xffffu);
+    vb = scale_byte(top >> 16);
+    const f2 mi = dup(scale_inverse(mb)), vi = dup(scale_inverse(vb));
+    const uint32_t r0 = round_bits(i0 / 4, e.key, 0u), r1 = round_bits(i0 / 4 + 1, e.key, 0u);
+    f2 y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = mul(m[k], mi);
+    store_codes<FULL>((uint8_t*)e.m + i0, encode8(y, r0, r1), n);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = mul(v[k], vi);
+    uint2 c = encode8(y, r0, r1);
+    // a second moment beside one that is not zero is held at no less than the smallest code:
+    // a byte c + 0x7f has its top bit clear only for c = 0
+    if (top >= 0x10000u) {
+      c.x |= (~(c.x + 0x7f7f7f7fu) & 0x80808080u) >> 7;
+      c.y |= (~(c.y + 0x7f7f7f7fu) & 0x80808080u) >> 7;
+    }
+    store_codes<FULL>((uint8_t*)e.v + i0, c, n);
+  } else {
+    values(in.m, m);
+    values(in.v, v);
+    const f2 b2 = dup(sc.beta2), neg = dup(-1.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      m[k] = add(m[k], mul(fma(m[k], neg, g[k]), w1));
+      v[k] = add(mul(v[k], b2), mul(mul(g[k], g[k]), w2));
+    }
+    store8<FULL>((float*)e.m + i0, m, n);
+    store8<FULL>((float*)e.v + i0, v, n);
+  }
+  if (e.p == nullptr) return;
+  if (!e.degenerate) {
+    const f2 c = dup(e.c);
+    if (e.eps == 0.f) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m[k] = angle2(mul(m[k], c), v[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a, b;
+        unpack_f2(v[k], a, b);
+        m[k] = mul(mul(m[k], c), pack_f2(rcp_approx(sqrt_approx(a) + e.eps), rcp_approx(sqrt_approx(b) + e.eps)));
+      }
+    }
+  }
+  f2 w[4];
+  values(in.w, w);
+  const f2 lr = dup(-e.lr);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (sc.wd > 0.f) {
+      float u0, u1, w0, w1_, s0, s1;
+      unpack_f2(m[k], u0, u1);
+      unpack_f2(w[k], w0, w1_);
+      unpack_f2(mul(m[k], w[k]), s0, s1);
+      if (s0 >= 0.f) u0 = fmaf(sc.wd, w0, u0);
+      if (s1 >= 0.f) u1 = fmaf(sc.wd, w1_, u1);
+      m[k] = pack_f2(u0, u1);
+    }
+    w[k] = fma(lr, m[k], w[k]);
+  }
+  if constexpr (MASTER) store8<FULL>(e.w + i0, w, n);
+  store8<FULL>((P*)e.p + i0, w, n);
+}
+
 // S8: moments in 8 bits, else fp32.  MASTER: the update is applied to fp32 master weights
 // and p receives their rounding.
 template <class P, bool S8, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kStThreads) adamw_state_kernel(const __grid_constant__ StAdamArgs<CAP> a) {
-  using W = std::conditional_t<MASTER, float, P>;
   const int ti = st_find(a.tb, blockIdx.x);
   const StAdam& e = a.tb.t[ti];
   const int64_t base = int64_t(blockIdx.x - a.tb.start[ti]) * kStChunk;
-  const P* G = (const P*)e.g;
-  W* Wp = MASTER ? (W*)e.w : (W*)e.p;
-  const bool apply = e.p != nullptr;
-  const int lane = threadIdx.x & 31;
+  const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8;
+  using In = AdamIn<P, S8, MASTER>;
+  if (e.vec && base + kStChunk <= e.numel) {
+    uint32_t ms = 0u, vs = 0u;
+    if constexpr (S8) {
+      ms = load_seg_bytes(e.ms + seg / kQBlock);
+      vs = load_seg_bytes(e.vs + seg / kQBlock);
+    }
+    uint32_t mout = 0u, vout = 0u;
+    In in;
+    adam_load<true>(e, i0, 8, in);
+#pragma unroll
+    for (int it = 0; it < kStIter; ++it) {
+      In next;
+      if (it + 1 < kStIter) adam_load<true>(e, i0 + (it + 1) * 256, 8, next);
+      uint32_t mb = seg_byte(ms, it), vb = seg_byte(vs, it);
+      adam_step8<true>(e, a.s, i0 + it * 256, 8, in, mb, vb);
+      mout |= mb << (8 * it);
+      vout |= vb << (8 * it);
+      in = next;
+    }
+    if constexpr (S8) {
+      store_seg_bytes(e.ms + seg / kQBlock, mout);
+      store_seg_bytes(e.vs + seg / kQBlock, vout);
+    }
+  } else {
 #pragma unroll 1
-  for (int it = 0; it < kStChunk / kStStep; ++it) {
-    const int64_t i0 = base + it * kStStep + threadIdx.x * 8;
-    if (base + it * kStStep >= e.numel) break;
-    const int n = (int)max64(0, min64(8, e.numel - i0));
-    const bool full = e.vec && n == 8;
-    float gv[8], mv[8], vv[8], wv[8];
-    unpack_raw(load_raw(G + i0, n, full), gv);
-    if constexpr (S8) {
-      const uint8_t* M = (const uint8_t*)e.m;
-      const uint8_t* V = (const uint8_t*)e.v;
-      const uint2 mc = load_codes(M + i0, n, full), vc = load_codes(V + i0, n, full);
-      const float ms = scale_value(n > 0 ? e.ms[i0 / kQBlock] : 0u), vs = scale_value(n > 0 ? e.vs[i0 / kQBlock] : 0u);
-      decode8(mc, mv);
-      decode8(vc, vv);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        mv[k] = k < n ? mv[k] * ms : 0.f;
-        vv[k] = k < n ? vv[k] * vs : 0.f;
+    for (int it = 0; it < kStIter && seg + it * 256 < e.numel; ++it) {
+      const int64_t i = i0 + it * 256;
+      const int n = (int)max64(0, min64(8, e.numel - i));
+      In in;
+      adam_load<false>(e, i, n, in);
+      uint32_t mb = 0u, vb = 0u;
+      if (S8 && n > 0) {
+        mb = e.ms[i / kQBlock];
+        vb = e.vs[i / kQBlock];
       }
-    } else {
-      unpack_raw(load_raw((const float*)e.m + i0, n, full), mv);
-      unpack_raw(load_raw((const float*)e.v + i0, n, full), vv);
-    }
-    if (apply) unpack_raw(load_raw(Wp + i0, n, full), wv);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      mv[k] = __fadd_rn(mv[k], __fmul_rn(__fsub_rn(gv[k], mv[k]), a.s.w1));
-      vv[k] = __fadd_rn(__fmul_rn(vv[k], a.s.beta2), __fmul_rn(__fmul_rn(gv[k], gv[k]), a.s.w2));
-    }
-    if constexpr (S8) {
-      uint32_t top = top16(mv) | (top16(vv) << 16);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const uint32_t mb = scale_byte(top & 0xffffu), vb = scale_byte(top >> 16);
-      const float mi = scale_inverse(mb), vi = scale_inverse(vb);
-      const float low = (top >> 16) != 0u ? 0.001953125f : 0.f;  // the smallest code, 2^-9
-      uint32_t mc[2], vc[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t r = round_bits(i0 / 4 + h, e.key, 0u);
-        float y[4], z[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          y[k] = mv[4 * h + k] * mi;
-          z[k] = fmaxf(vv[4 * h + k] * vi, low);
-        }
-        mc[h] = encode4(y[0], y[1], y[2], y[3], r);
-        vc[h] = encode4(z[0], z[1], z[2], z[3], r);
+      adam_step8<false>(e, a.s, i, n, in, mb, vb);
+      if (S8 && n > 0 && (threadIdx.x & 15) == 0) {
+        e.ms[i / kQBlock] = (uint8_t)mb;
+        e.vs[i / kQBlock] = (uint8_t)vb;
       }
-      store_codes((uint8_t*)e.m + i0, make_uint2(mc[0], mc[1]), n, full);
-      store_codes((uint8_t*)e.v + i0, make_uint2(vc[0], vc[1]), n, full);
-      if ((lane & 15) == 0 && n > 0) {
-        e.ms[i0 / kQBlock] = (uint8_t)mb;
-        e.vs[i0 / kQBlock] = (uint8_t)vb;
-      }
-    } else {
-      store_n((float*)e.m + i0, mv, n, e.vec);
-      store_n((float*)e.v + i0, vv, n, e.vec);
-    }
-    if (apply) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float u;
-        if (e.degenerate) u = mv[k];
-        else if (a.s.eps == 0.f) u = atan2f(mv[k] * e.bc1, sqrtf(vv[k] * e.bc2));
-        else u = (mv[k] * e.bc1) / (sqrtf(vv[k] * e.bc2) + a.s.eps);
-        if (a.s.wd > 0.f && u * wv[k] >= 0.f) u = u + a.s.wd * wv[k];
-        wv[k] = wv[k] - e.lr * u;
-      }
-      if (MASTER) store_n(e.w + i0, wv, n, e.vec);
-      store_n((P*)e.p + i0, wv, n, e.vec);
     }
   }
 }
@@ -346,9 +557,45 @@ struct StMomentumArgs {
   float beta1;
 };
 
-__device__ __forceinline__ void momentum_u8(const float* g, const float* m, float b1, float* u) {
+// One matrix of a tensor.
+template <class P>
+struct StMatrix {
+  const P* g;
+  uint8_t* m;
+  uint8_t* ms;
+};
+template <class P>
+__device__ __forceinline__ StMatrix<P> matrix_of(const StMomentum& e, int64_t b) {
+  return StMatrix<P>{(const P*)e.g + b * e.run, e.m + b * e.run, e.ms + b * ((e.run + kQBlock - 1) / kQBlock)};
+}
+
+// Momentum of one thread's 8 elements, mb as above; adds the squares of u = g + beta1 m.
+template <bool FULL, class P>
+__device__ __forceinline__ f2 momentum_step8(const StMatrix<P>& t, int64_t i0, int n, const Raw8<P>& graw, uint2 c,
+                                             uint32_t& mb, float beta1, uint64_t key, uint32_t run, f2 sq) {
+  f2 g[4], m[4], y[4];
+  values(graw, g);
+  decode8(c, m);
+  const f2 s = dup(scale_value(mb) * beta1);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) u[k] = __fadd_rn(g[k], __fmul_rn(m[k], b1));
+  for (int k = 0; k < 4; ++k) m[k] = add(mul(m[k], s), g[k]);
+  uint32_t top = top16(m);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  mb = scale_byte(top);
+  const f2 inv = dup(scale_inverse(mb));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) y[k] = mul(m[k], inv);
+  c = encode8(y, round_bits(i0 / 4, key, run), round_bits(i0 / 4 + 1, key, run));
+  store_codes<FULL>(t.m + i0, c, n);
+  decode8(c, m);
+  const f2 s2 = dup(scale_value(mb) * beta1);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const f2 u = add(g[k], mul(m[k], s2));
+    sq = fma(u, u, sq);
+  }
+  return sq;
 }
 
 template <class P, int CAP>
@@ -358,46 +605,42 @@ __global__ void __launch_bounds__(kStThreads) momentum8_kernel(const __grid_cons
   const StMomentum& e = a.tb.t[ti];
   const int64_t local = blockIdx.x - a.tb.start[ti];
   const int64_t b = local / e.chunks, base = (local - b * e.chunks) * kStChunk;
-  const P* G = (const P*)e.g + b * e.run;
-  uint8_t* M = e.m + b * e.run;
-  uint8_t* MS = e.ms + b * ((e.run + kQBlock - 1) / kQBlock);
-  const int lane = threadIdx.x & 31;
-  float sq = 0.f;
+  const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8;
+  const StMatrix<P> t = matrix_of<P>(e, b);
+  f2 sq = dup(0.f);
+  if (e.vec && base + kStChunk <= e.run) {
+    Raw8<P> g[kStIter];
+    uint2 c[kStIter];
+#pragma unroll
+    for (int it = 0; it < kStIter; ++it) {
+      load_raw<true>(t.g + i0 + it * 256, 8, g[it]);
+      c[it] = load_codes<true>(t.m + i0 + it * 256, 8);
+    }
+    const uint32_t ms = load_seg_bytes(t.ms + seg / kQBlock);
+    uint32_t out = 0u;
+#pragma unroll
+    for (int it = 0; it < kStIter; ++it) {
+      uint32_t mb = seg_byte(ms, it);
+      sq = momentum_step8<true>(t, i0 + it * 256, 8, g[it], c[it], mb, a.beta1, e.key, (uint32_t)b, sq);
+      out |= mb << (8 * it);
+    }
+    store_seg_bytes(t.ms + seg / kQBlock, out);
+  } else {
 #pragma unroll 1
-  for (int it = 0; it < kStChunk / kStStep; ++it) {
-    const int64_t i0 = base + it * kStStep + threadIdx.x * 8;
-    if (base + it * kStStep >= e.run) break;
-    const int n = (int)max64(0, min64(8, e.run - i0));
-    const bool full = e.vec && n == 8;
-    float gv[8], mv[8], u[8];
-    unpack_raw(load_raw(G + i0, n, full), gv);
-    const uint2 mc = load_codes(M + i0, n, full);
-    const float ms = scale_value(n > 0 ? MS[i0 / kQBlock] : 0u);
-    decode8(mc, mv);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      mv[k] = k < n ? __fadd_rn(__fmul_rn(mv[k] * ms, a.beta1), gv[k]) : 0.f;
-    uint32_t top = top16(mv);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const uint32_t mb = scale_byte(top);
-    const float mi = scale_inverse(mb);
-    uint2 c;
-    c.x = encode4(mv[0] * mi, mv[1] * mi, mv[2] * mi, mv[3] * mi, round_bits(i0 / 4, e.key, (uint32_t)b));
-    c.y = encode4(mv[4] * mi, mv[5] * mi, mv[6] * mi, mv[7] * mi, round_bits(i0 / 4 + 1, e.key, (uint32_t)b));
-    store_codes(M + i0, c, n, full);
-    if ((lane & 15) == 0 && n > 0) MS[i0 / kQBlock] = (uint8_t)mb;
-    decode8(c, mv);
-    const float mn = scale_value(mb);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) mv[k] *= mn;
-    momentum_u8(gv, mv, a.beta1, u);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < n) sq = __fmaf_rn(u[k], u[k], sq);
+    for (int it = 0; it < kStIter && seg + it * 256 < e.run; ++it) {
+      const int64_t i = i0 + it * 256;
+      const int n = (int)max64(0, min64(8, e.run - i));
+      Raw8<P> g;
+      load_raw<false>(t.g + i, n, g);
+      uint32_t mb = n > 0 ? t.ms[i / kQBlock] : 0u;
+      sq = momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, a.beta1, e.key, (uint32_t)b, sq);
+      if (n > 0 && (threadIdx.x & 15) == 0) t.ms[i / kQBlock] = (uint8_t)mb;
+    }
   }
   if (e.x != nullptr) {
-    const float tot = block_sum(sq, red);
+    float s0, s1;
+    unpack_f2(sq, s0, s1);
+    const float tot = block_sum(s0 + s1, red);
     if (threadIdx.x == 0) e.norm[e.batch + local] = tot;
   }
 }
@@ -416,45 +659,64 @@ __global__ void __launch_bounds__(kStThreads) momentum8_norm_kernel(const __grid
   if (threadIdx.x == 0) e.norm[b] = sqrtf((float)s);
 }
 
+template <bool FULL, class P, class X>
+__device__ __forceinline__ void input_step8(const StMomentum& e, X* xb, int64_t i0, int n, const Raw8<P>& graw, uint2 c,
+                                            uint32_t mb, float beta1, float inv1) {
+  f2 g[4], m[4];
+  values(graw, g);
+  decode8(c, m);
+  const f2 s = dup(scale_value(mb) * beta1), inv = dup(inv1);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) m[k] = mul(add(g[k], mul(m[k], s)), inv);
+  if (FULL || e.ldx == e.cols) {
+    store8<FULL>(xb + i0, m, n);
+  } else {  // rows padded to a longer leading dimension
+    float u[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) unpack_f2(m[k], u[2 * k], u[2 * k + 1]);
+    int64_t r = i0 / e.cols, col = i0 - r * e.cols;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k < n) xb[r * e.ldx + col] = from_f<X>(u[k]);
+      if (++col == e.cols) {
+        col = 0;
+        ++r;
+      }
+    }
+  }
+}
+
 template <class P, class X, int CAP>
 __global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
   const int ti = st_find(a.tb, blockIdx.x);
   const StMomentum& e = a.tb.t[ti];
   const int64_t local = blockIdx.x - a.tb.start[ti];
   const int64_t b = local / e.chunks, base = (local - b * e.chunks) * kStChunk;
-  const P* G = (const P*)e.g + b * e.run;
-  const uint8_t* M = e.m + b * e.run;
-  const uint8_t* MS = e.ms + b * ((e.run + kQBlock - 1) / kQBlock);
-  const int64_t rows = e.run / e.cols;
-  X* xb = (X*)e.x + b * rows * e.ldx;
+  const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8;
+  const StMatrix<P> t = matrix_of<P>(e, b);
+  X* xb = (X*)e.x + b * (e.run / e.cols) * e.ldx;
   const float inv = 1.f / (e.norm[b] + 1e-8f);
+  if (e.vec && e.ldx == e.cols && base + kStChunk <= e.run) {
+    Raw8<P> g[kStIter];
+    uint2 c[kStIter];
+#pragma unroll
+    for (int it = 0; it < kStIter; ++it) {
+      load_raw<true>(t.g + i0 + it * 256, 8, g[it]);
+      c[it] = load_codes<true>(t.m + i0 + it * 256, 8);
+    }
+    const uint32_t ms = load_seg_bytes(t.ms + seg / kQBlock);
+#pragma unroll
+    for (int it = 0; it < kStIter; ++it)
+      input_step8<true>(e, xb, i0 + it * 256, 8, g[it], c[it], seg_byte(ms, it), a.beta1, inv);
+  } else {
 #pragma unroll 1
-  for (int it = 0; it < kStChunk / kStStep; ++it) {
-    const int64_t i0 = base + it * kStStep + threadIdx.x * 8;
-    const int n = (int)max64(0, min64(8, e.run - i0));
-    if (n == 0) break;
-    const bool full = e.vec && n == 8;
-    float gv[8], mv[8], u[8];
-    unpack_raw(load_raw(G + i0, n, full), gv);
-    decode8(load_codes(M + i0, n, full), mv);
-    const float ms = scale_value(MS[i0 / kQBlock]);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) mv[k] *= ms;
-    momentum_u8(gv, mv, a.beta1, u);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) u[k] *= inv;
-    if (e.ldx == e.cols) {
-      store_n(xb + i0, u, n, e.vec);
-    } else {  // rows padded to a longer leading dimension
-      int64_t r = i0 / e.cols, c = i0 - r * e.cols;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (k < n) xb[r * e.ldx + c] = from_f<X>(u[k]);
-        if (++c == e.cols) {
-          c = 0;
-          ++r;
-        }
-      }
+    for (int it = 0; it < kStIter; ++it) {
+      const int64_t i = i0 + it * 256;
+      const int n = (int)max64(0, min64(8, e.run - i));
+      if (n == 0) break;
+      Raw8<P> g;
+      load_raw<false>(t.g + i, n, g);
+      input_step8<false>(e, xb, i, n, g, load_codes<false>(t.m + i, n), t.ms[i / kQBlock], a.beta1, inv);
     }
   }
 }
@@ -480,46 +742,67 @@ struct StApplyArgs {
 
 constexpr float kF32Eps = 1.1920928955078125e-07f;  // the master weights' type
 
+template <class U, class P, bool FULL>
+__device__ __forceinline__ void apply_step8(const StApply& e, float wd, int64_t i0, int n) {
+  f2 u[4], w[4];
+  Raw8<U> ur;
+  Raw8<float> wr;
+  load_raw<FULL>((const U*)e.U + i0, n, ur);
+  load_raw<FULL>((const float*)e.w + i0, n, wr);
+  values(ur, u);
+  values(wr, w);
+  float uv[8], wv[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    unpack_f2(u[k], uv[2 * k], uv[2 * k + 1]);
+    unpack_f2(w[k], wv[2 * k], wv[2 * k + 1]);
+  }
+  if (e.row_scale != nullptr) {
+    int64_t r = i0 / e.cols, c = i0 - r * e.cols;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (FULL || k < n) {
+        float s = e.row_scale[r];
+        if (e.mat_stats != nullptr) {
+          const int64_t b = r / e.rows;
+          s *= sqrtf(e.mat_stats[2 * b]) / fmaxf(sqrtf(e.mat_stats[2 * b + 1]), kF32Eps);
+        }
+        uv[k] *= s;
+      }
+      if (++c == e.cols) {
+        c = 0;
+        ++r;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (wd > 0.f && uv[k] * wv[k] >= 0.f) uv[k] = fmaf(wd, wv[k], uv[k]);
+    wv[k] = fmaf(-e.lr, uv[k], wv[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = pack_f2(wv[2 * k], wv[2 * k + 1]);
+  store8<FULL>(e.w + i0, w, n);
+  store8<FULL>((P*)e.p + i0, w, n);
+}
+
 template <class U, class P, int CAP>
 __global__ void __launch_bounds__(kStThreads) apply_master_kernel(const __grid_constant__ StApplyArgs<CAP> a) {
   const int ti = st_find(a.tb, blockIdx.x);
   const StApply& e = a.tb.t[ti];
   const int64_t base = int64_t(blockIdx.x - a.tb.start[ti]) * kStChunk;
+  if (e.vec && base + kStChunk <= e.numel) {
 #pragma unroll 1
-  for (int it = 0; it < kStChunk / kStStep; ++it) {
-    const int64_t i0 = base + it * kStStep + threadIdx.x * 8;
-    const int n = (int)max64(0, min64(8, e.numel - i0));
-    if (n == 0) break;
-    const bool full = e.vec && n == 8;
-    float uv[8], wv[8];
-    unpack_raw(load_raw((const U*)e.U + i0, n, full), uv);
-    unpack_raw(load_raw((const float*)e.w + i0, n, full), wv);
-    if (e.row_scale != nullptr) {
-      int64_t r = i0 / e.cols, c = i0 - r * e.cols;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (k < n) {
-          float s = e.row_scale[r];
-          if (e.mat_stats != nullptr) {
-            const int64_t b = r / e.rows;
-            s *= sqrtf(e.mat_stats[2 * b]) / fmaxf(sqrtf(e.mat_stats[2 * b + 1]), kF32Eps);
-          }
-          uv[k] *= s;
-        }
-        if (++c == e.cols) {
-          c = 0;
-          ++r;
-        }
-      }
+    for (int it = 0; it < kStChunk / kStStep; ++it)
+      apply_step8<U, P, true>(e, a.wd, base + it * kStStep + threadIdx.x * 8, 8);
+  } else {
+#pragma unroll 1
+    for (int it = 0; it < kStChunk / kStStep; ++it) {
+      const int64_t i0 = base + it * kStStep + threadIdx.x * 8;
+      const int n = (int)max64(0, min64(8, e.numel - i0));
+      if (n == 0) break;
+      apply_step8<U, P, false>(e, a.wd, i0, n);
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      float u = uv[k];
-      if (a.wd > 0.f && u * wv[k] >= 0.f) u = u + a.wd * wv[k];
-      wv[k] = wv[k] - e.lr * u;
-    }
-    store_n(e.w + i0, wv, n, e.vec);
-    store_n((P*)e.p + i0, wv, n, e.vec);
   }
 }
 
@@ -540,13 +823,14 @@ static int64_t st_elems(int64_t b, int64_t r, int64_t c) {
 }
 
 template <class P, bool S8, bool MASTER>
-static int adam_launch(const thorn_adamw_state_tensor* ts, int n, const StAdamScalars& sc, cudaStream_t st) {
+static int adam_launch(const thorn_adamw_state_tensor* ts, int n, const StAdamScalars& sc, float eps, cudaStream_t st) {
   return st_launch<StAdam, kStCap>(
       ts, n,
-      [](const thorn_adamw_state_tensor& t, StAdam& e) -> int64_t {
+      [eps](const thorn_adamw_state_tensor& t, StAdam& e) -> int64_t {
         if ((t.w != nullptr) != MASTER) return 0;
+        const double root = sqrt((double)t.bc2);
         e = StAdam{t.p, t.g, (float*)t.w, t.m, t.v, (uint8_t*)t.m_scale, (uint8_t*)t.v_scale, t.numel,
-                   rounding_key(t.seed), t.lr, t.bc1, t.bc2, t.degenerate, 0};
+                   rounding_key(t.seed), t.lr, (float)(t.bc1 / root), (float)(eps / root), t.degenerate, 0};
         const bool mv = S8 ? aligned8(t.m) && aligned8(t.v) : aligned16(t.m) && aligned16(t.v);
         e.vec = mv && aligned16(t.g) && aligned16(t.p) && aligned16(t.w);
         return st_cdiv(t.numel, kStChunk);
@@ -563,8 +847,8 @@ static int adam_launch(const thorn_adamw_state_tensor* ts, int n, const StAdamSc
 
 using namespace thorn;
 
-static StAdamScalars adam_scalars(double beta1, double beta2, float wd, float eps) {
-  return StAdamScalars{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), wd, eps};
+static StAdamScalars adam_scalars(double beta1, double beta2, float wd) {
+  return StAdamScalars{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), wd};
 }
 
 extern "C" int thorn_adamw8_multi(const thorn_adamw_state_tensor* ts, int n, int p_dtype, double beta1, double beta2,
@@ -576,16 +860,16 @@ extern "C" int thorn_adamw8_multi(const thorn_adamw_state_tensor* ts, int n, int
     if (t.numel > 0 && (!t.g || !t.m || !t.v || !t.m_scale || !t.v_scale)) return THORN_ERR_ARG;
     if (t.w && p_dtype == THORN_F32) return THORN_ERR_ARG;
   }
-  const StAdamScalars sc = adam_scalars(beta1, beta2, weight_decay, eps);
+  const StAdamScalars sc = adam_scalars(beta1, beta2, weight_decay);
   cudaStream_t st = (cudaStream_t)stream;
-  if (p_dtype == THORN_F32) return adam_launch<float, true, false>(ts, n, sc, st);
+  if (p_dtype == THORN_F32) return adam_launch<float, true, false>(ts, n, sc, eps, st);
   int rc;
   if (p_dtype == THORN_BF16) {
-    rc = adam_launch<__nv_bfloat16, true, false>(ts, n, sc, st);
-    return rc ? rc : adam_launch<__nv_bfloat16, true, true>(ts, n, sc, st);
+    rc = adam_launch<__nv_bfloat16, true, false>(ts, n, sc, eps, st);
+    return rc ? rc : adam_launch<__nv_bfloat16, true, true>(ts, n, sc, eps, st);
   }
-  rc = adam_launch<__half, true, false>(ts, n, sc, st);
-  return rc ? rc : adam_launch<__half, true, true>(ts, n, sc, st);
+  rc = adam_launch<__half, true, false>(ts, n, sc, eps, st);
+  return rc ? rc : adam_launch<__half, true, true>(ts, n, sc, eps, st);
 }
 
 extern "C" int thorn_adamw_master_multi(const thorn_adamw_state_tensor* ts, int n, int p_dtype, double beta1,
@@ -596,10 +880,10 @@ extern "C" int thorn_adamw_master_multi(const thorn_adamw_state_tensor* ts, int 
     if (t.numel < 0 || t.numel > kStMaxElems) return THORN_ERR_ARG;
     if (t.numel > 0 && (!t.g || !t.m || !t.v || !t.w)) return THORN_ERR_ARG;
   }
-  const StAdamScalars sc = adam_scalars(beta1, beta2, weight_decay, eps);
+  const StAdamScalars sc = adam_scalars(beta1, beta2, weight_decay);
   cudaStream_t st = (cudaStream_t)stream;
-  if (p_dtype == THORN_BF16) return adam_launch<__nv_bfloat16, false, true>(ts, n, sc, st);
-  return adam_launch<__half, false, true>(ts, n, sc, st);
+  if (p_dtype == THORN_BF16) return adam_launch<__nv_bfloat16, false, true>(ts, n, sc, eps, st);
+  return adam_launch<__half, false, true>(ts, n, sc, eps, st);
 }
 
 extern "C" int64_t thorn_momentum8_scratch_bytes(int64_t batch, int64_t rows, int64_t cols) {
