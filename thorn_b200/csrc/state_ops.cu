@@ -94,13 +94,23 @@ __device__ __forceinline__ uint32_t mul_fold(uint32_t a, uint32_t b) {
   return (uint32_t)(t >> 32) ^ (uint32_t)t;
 }
 
-// 32 random bits for elements 4q .. 4q+3 of run `run`: a Weyl sequence through two
-// multiply-and-fold rounds (7 integer instructions for four elements).
-__device__ __forceinline__ uint32_t round_bits(int64_t q, uint64_t key, uint32_t run) {
-  const uint32_t a = (uint32_t)q * 0x9E3779B9u + (uint32_t)key;
-  const uint32_t x = mul_fold(a, a ^ ((uint32_t)(key >> 32) ^ ((uint32_t)(q >> 32) + run)));
-  return mul_fold(x, x ^ 0xBB67AE85u);
-}
+// 32 random bits for elements 4q .. 4q+3 of a run: a Weyl sequence through two
+// multiply-and-fold rounds.  q's upper half and the run enter the second word of the key,
+// which a chunk's elements share.
+struct Rounding {
+  uint32_t a, k;
+  __device__ __forceinline__ Rounding(int64_t i0, uint64_t key, uint32_t run) {
+    const uint64_t q = (uint64_t)i0 >> 2;
+    a = (uint32_t)q * 0x9E3779B9u + (uint32_t)key;
+    k = (uint32_t)(key >> 32) ^ ((uint32_t)(q >> 32) + run);
+  }
+  // for the four elements that follow `step` times four others
+  __device__ __forceinline__ uint32_t bits(uint32_t step) const {
+    const uint32_t w = a + step * 0x9E3779B9u;
+    const uint32_t x = mul_fold(w, w ^ k);
+    return mul_fold(x, x ^ 0xBB67AE85u);
+  }
+};
 
 // Four values -> four e4m3 codes (element 0 in the low byte), each rounded up in magnitude
 // with the probability of its distance to the lower neighbour.  The instruction takes 16
@@ -166,14 +176,8 @@ __device__ __forceinline__ uint2 encode8(const f2* y, uint32_t r0, uint32_t r1) 
   return o;
 }
 
-// 2^(b - 127), NaN for b = 255
-__device__ __forceinline__ float scale_value(uint32_t b) {
-  return __uint_as_float(b == 255u ? 0x7fc00000u : (b == 0u ? 0x00400000u : b << 23));
-}
-// 2^(127 - b), NaN for b = 255
-__device__ __forceinline__ float scale_inverse(uint32_t b) {
-  return __uint_as_float(b == 255u ? 0x7fc00000u : (254u - b) << 23);
-}
+// 2^(b - 127); infinity for b = 255, whose codes are NaN
+__device__ __forceinline__ float scale_value(uint32_t b) { return __uint_as_float(max(b << 23, 0x00400000u)); }
 
 // The upper 16 bits of max|v| of 8 values, rounded up: enough for the block's scale (the
 // only mantissa it is compared with is 1.75), and two of them fit one shuffle.  A NaN
@@ -191,11 +195,14 @@ __device__ __forceinline__ uint32_t top16(const f2* v) {
   return (__float_as_uint(t) + 0xffffu) >> 16;
 }
 
-// Scale byte of a block from its top16: the smallest power of two with max <= 448 * 2^k
-// (448 = 1.75 * 2^8 is the largest e4m3 value); 255 for a block that is not finite.
-__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
-  const int b = max((int)((top + 0x1fu) >> 7) - 8, 0);
-  return top >= 0x7f80u ? 255u : (uint32_t)b;
+// Scale byte b of a block from its top16, the smallest power of two with max <= 448 * 2^k
+// (448 = 1.75 * 2^8 is the largest e4m3 value), and 2^(127 - b).  A block that is not finite
+// gets 255 and NaN, which makes all its codes NaN.
+__device__ __forceinline__ uint32_t block_scale(uint32_t top, float& inverse) {
+  const uint32_t b = (uint32_t)max((int)((top + 0x1fu) >> 7) - 8, 0);
+  const bool finite = top < 0x7f80u;
+  inverse = __uint_as_float(finite ? (254u - b) << 23 : 0x7fc00000u);
+  return finite ? b : 255u;
 }
 
 // ---------------------------------------------------------------------------
@@ -284,6 +291,9 @@ __device__ __forceinline__ uint32_t load_seg_bytes(const uint8_t* p) {
   return p[half] | (uint32_t)p[2 + half] << 8 | (uint32_t)p[4 + half] << 16 | (uint32_t)p[6 + half] << 24;
 }
 __device__ __forceinline__ uint32_t seg_byte(uint32_t b, int it) { return (b >> (8 * it)) & 0xffu; }
+__device__ __forceinline__ uint32_t put_byte(uint32_t w, uint32_t b, int it) {
+  return __byte_perm(w, b, it == 0 ? 0x3214 : (it == 1 ? 0x3240 : (it == 2 ? 0x3410 : 0x4210)));
+}
 __device__ __forceinline__ void store_seg_bytes(uint8_t* p, uint32_t b) {
   const uint32_t o = __shfl_xor_sync(0xffffffffu, b, 16);
   if ((threadIdx.x & 31) == 0) {
@@ -316,20 +326,21 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return r;
 }
 
-// atan2(y, sqrt(x2)) of two elements, x2 >= 0: the angle of t = |y| / sqrt(x2), from t or
-// 1/t in [0, 1].  x2 is taken 2^-126 higher (nothing in fp32 from 2^-102 up), so that zero
-// over zero is zero and a subnormal x2 needs no case of its own; it acts like an eps of
-// 1e-19 beside the root.  The polynomial in s^2 is the minimax fit of atan(s)/s on [0, 1]
-// with eight coefficients (Remez exchange: 9.9e-8 relative, 2.1e-7 with the roundings of
-// its fp32 evaluation).  The general function, with an exact square root and divisions,
-// made the 8-bit step of two 128256 x 4096 tensors 4108 us where this makes it 3103.
+// atan2(y, sqrt(x2)) of two elements, x2 >= 0: with t = y / sqrt(x2), atan(s) for s = t where
+// |t| <= 1, else +-pi/2 + atan(s) for s = -1/t.  x2 is taken 2^-126 higher (nothing in fp32
+// from 2^-102 up), so that zero over zero is zero and a subnormal x2 needs no case of its
+// own; it acts like an eps of 1e-19 beside the root.  The polynomial in s^2 is the minimax
+// fit of atan(s)/s on [0, 1] with eight coefficients (Remez exchange: 9.9e-8 relative,
+// 2.1e-7 with the roundings of its fp32 evaluation).  The general function, with an exact
+// square root and divisions, made the first 8-bit step of two 128256 x 4096 tensors 4108 us
+// where this made it 3103.
 __device__ __forceinline__ f2 angle2(f2 y, f2 x2) {
-  float y0, y1, q0, q1;
-  unpack_f2(y, y0, y1);
+  float t0, t1, q0, q1;
   unpack_f2(add(x2, dup(1.17549435e-38f)), q0, q1);
-  const float t0 = fabsf(y0) * rsqrt_approx(q0), t1 = fabsf(y1) * rsqrt_approx(q1);
-  const bool b0 = t0 > 1.f, b1 = t1 > 1.f;
-  const f2 s = pack_f2(b0 ? rcp_approx(t0) : t0, b1 ? rcp_approx(t1) : t1);
+  unpack_f2(mul(y, pack_f2(rsqrt_approx(q0), rsqrt_approx(q1))), t0, t1);
+  const bool b0 = fabsf(t0) > 1.f, b1 = fabsf(t1) > 1.f;
+  const f2 s = pack_f2(b0 ? rcp_approx(-t0) : t0, b1 ? rcp_approx(-t1) : t1);
+  const f2 r = pack_f2(b0 ? copysignf(1.57079632679f, t0) : 0.f, b1 ? copysignf(1.57079632679f, t1) : 0.f);
   const f2 z = mul(s, s);
   f2 p = dup(-0.0046932776f);
   p = fma(p, z, dup(0.02425241f));
@@ -339,11 +350,7 @@ __device__ __forceinline__ f2 angle2(f2 y, f2 x2) {
   p = fma(p, z, dup(0.19969724f));
   p = fma(p, z, dup(-0.3333199f));
   p = fma(p, z, dup(0.9999999f));
-  float a0, a1;
-  unpack_f2(mul(s, p), a0, a1);
-  a0 = b0 ? 1.57079632679f - a0 : a0;
-  a1 = b1 ? 1.57079632679f - a1 : a1;
-  return pack_f2(copysignf(a0, y0), copysignf(a1, y1));
+  return fma(s, p, r);
 }
 
 // ===========================================================================
@@ -401,7 +408,8 @@ __device__ __forceinline__ void adam_load(const StAdam& e, int64_t i0, int n, Ad
 // the power-of-two scales inside the fmas are exact).
 template <bool FULL, class P, bool S8, bool MASTER>
 __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars& sc, int64_t i0, int n,
-                                           const AdamIn<P, S8, MASTER>& in, uint32_t& mb, uint32_t& vb) {
+                                           const AdamIn<P, S8, MASTER>& in, const Rounding& rnd, uint32_t step,
+                                           uint32_t& mb, uint32_t& vb) {
   f2 g[4], m[4], v[4];
   const f2 w1 = dup(sc.w1), w2 = dup(sc.w2);
   values(in.g, g);
@@ -418,10 +426,11 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
     uint32_t top = top16(m) | (top16(v) << 16);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-    mb = scale_byte(top & 0xffffu);
-    vb = scale_byte(top >> 16);
-    const f2 mi = dup(scale_inverse(mb)), vi = dup(scale_inverse(vb));
-    const uint32_t r0 = round_bits(i0 / 4, e.key, 0u), r1 = round_bits(i0 / 4 + 1, e.key, 0u);
+    float mi1, vi1;
+    mb = block_scale(top & 0xffffu, mi1);
+    vb = block_scale(top >> 16, vi1);
+    const f2 mi = dup(mi1), vi = dup(vi1);
+    const uint32_t r0 = rnd.bits(step), r1 = rnd.bits(step + 1);
     f2 y[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) y[k] = mul(m[k], mi);
@@ -465,20 +474,17 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
   }
   f2 w[4];
   values(in.w, w);
+  if (sc.wd > 0.f) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float s0, s1;
+      unpack_f2(mul(m[k], w[k]), s0, s1);
+      m[k] = fma(pack_f2(s0 >= 0.f ? sc.wd : 0.f, s1 >= 0.f ? sc.wd : 0.f), w[k], m[k]);
+    }
+  }
   const f2 lr = dup(-e.lr);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (sc.wd > 0.f) {
-      float u0, u1, w0, w1_, s0, s1;
-      unpack_f2(m[k], u0, u1);
-      unpack_f2(w[k], w0, w1_);
-      unpack_f2(mul(m[k], w[k]), s0, s1);
-      if (s0 >= 0.f) u0 = fmaf(sc.wd, w0, u0);
-      if (s1 >= 0.f) u1 = fmaf(sc.wd, w1_, u1);
-      m[k] = pack_f2(u0, u1);
-    }
-    w[k] = fma(lr, m[k], w[k]);
-  }
+  for (int k = 0; k < 4; ++k) w[k] = fma(lr, m[k], w[k]);
   if constexpr (MASTER) store8<FULL>(e.w + i0, w, n);
   store8<FULL>((P*)e.p + i0, w, n);
 }
@@ -490,13 +496,14 @@ __global__ void __launch_bounds__(kStThreads) adamw_state_kernel(const __grid_co
   const int ti = st_find(a.tb, blockIdx.x);
   const StAdam& e = a.tb.t[ti];
   const int64_t base = int64_t(blockIdx.x - a.tb.start[ti]) * kStChunk;
-  const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8;
+  const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8, blk = seg >> 7;
   using In = AdamIn<P, S8, MASTER>;
+  const Rounding rnd(i0, e.key, 0u);
   if (e.vec && base + kStChunk <= e.numel) {
     uint32_t ms = 0u, vs = 0u;
     if constexpr (S8) {
-      ms = load_seg_bytes(e.ms + seg / kQBlock);
-      vs = load_seg_bytes(e.vs + seg / kQBlock);
+      ms = load_seg_bytes(e.ms + blk);
+      vs = load_seg_bytes(e.vs + blk);
     }
     uint32_t mout = 0u, vout = 0u;
     In in;
@@ -506,14 +513,14 @@ __global__ void __launch_bounds__(kStThreads) adamw_state_kernel(const __grid_co
       In next;
       if (it + 1 < kStIter) adam_load<true>(e, i0 + (it + 1) * 256, 8, next);
       uint32_t mb = seg_byte(ms, it), vb = seg_byte(vs, it);
-      adam_step8<true>(e, a.s, i0 + it * 256, 8, in, mb, vb);
-      mout |= mb << (8 * it);
-      vout |= vb << (8 * it);
+      adam_step8<true>(e, a.s, i0 + it * 256, 8, in, rnd, it * 64, mb, vb);
+      mout = put_byte(mout, mb, it);
+      vout = put_byte(vout, vb, it);
       in = next;
     }
     if constexpr (S8) {
-      store_seg_bytes(e.ms + seg / kQBlock, mout);
-      store_seg_bytes(e.vs + seg / kQBlock, vout);
+      store_seg_bytes(e.ms + blk, mout);
+      store_seg_bytes(e.vs + blk, vout);
     }
   } else {
 #pragma unroll 1
@@ -524,13 +531,13 @@ __global__ void __launch_bounds__(kStThreads) adamw_state_kernel(const __grid_co
       adam_load<false>(e, i, n, in);
       uint32_t mb = 0u, vb = 0u;
       if (S8 && n > 0) {
-        mb = e.ms[i / kQBlock];
-        vb = e.vs[i / kQBlock];
+        mb = e.ms[i >> 7];
+        vb = e.vs[i >> 7];
       }
-      adam_step8<false>(e, a.s, i, n, in, mb, vb);
+      adam_step8<false>(e, a.s, i, n, in, rnd, it * 64, mb, vb);
       if (S8 && n > 0 && (threadIdx.x & 15) == 0) {
-        e.ms[i / kQBlock] = (uint8_t)mb;
-        e.vs[i / kQBlock] = (uint8_t)vb;
+        e.ms[i >> 7] = (uint8_t)mb;
+        e.vs[i >> 7] = (uint8_t)vb;
       }
     }
   }
@@ -572,7 +579,7 @@ __device__ __forceinline__ StMatrix<P> matrix_of(const StMomentum& e, int64_t b)
 // Momentum of one thread's 8 elements, mb as above; adds the squares of u = g + beta1 m.
 template <bool FULL, class P>
 __device__ __forceinline__ f2 momentum_step8(const StMatrix<P>& t, int64_t i0, int n, const Raw8<P>& graw, uint2 c,
-                                             uint32_t& mb, float beta1, uint64_t key, uint32_t run, f2 sq) {
+                                             uint32_t& mb, float beta1, const Rounding& rnd, uint32_t step, f2 sq) {
   f2 g[4], m[4], y[4];
   values(graw, g);
   decode8(c, m);
@@ -582,11 +589,12 @@ __device__ __forceinline__ f2 momentum_step8(const StMatrix<P>& t, int64_t i0, i
   uint32_t top = top16(m);
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  mb = scale_byte(top);
-  const f2 inv = dup(scale_inverse(mb));
+  float inv1;
+  mb = block_scale(top, inv1);
+  const f2 inv = dup(inv1);
 #pragma unroll
   for (int k = 0; k < 4; ++k) y[k] = mul(m[k], inv);
-  c = encode8(y, round_bits(i0 / 4, key, run), round_bits(i0 / 4 + 1, key, run));
+  c = encode8(y, rnd.bits(step), rnd.bits(step + 1));
   store_codes<FULL>(t.m + i0, c, n);
   decode8(c, m);
   const f2 s2 = dup(scale_value(mb) * beta1);
@@ -605,8 +613,9 @@ __global__ void __launch_bounds__(kStThreads) momentum8_kernel(const __grid_cons
   const StMomentum& e = a.tb.t[ti];
   const int64_t local = blockIdx.x - a.tb.start[ti];
   const int64_t b = local / e.chunks, base = (local - b * e.chunks) * kStChunk;
-  const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8;
+  const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8, blk = seg >> 7;
   const StMatrix<P> t = matrix_of<P>(e, b);
+  const Rounding rnd(i0, e.key, (uint32_t)b);
   f2 sq = dup(0.f);
   if (e.vec && base + kStChunk <= e.run) {
     Raw8<P> g[kStIter];
@@ -616,15 +625,15 @@ __global__ void __launch_bounds__(kStThreads) momentum8_kernel(const __grid_cons
       load_raw<true>(t.g + i0 + it * 256, 8, g[it]);
       c[it] = load_codes<true>(t.m + i0 + it * 256, 8);
     }
-    const uint32_t ms = load_seg_bytes(t.ms + seg / kQBlock);
+    const uint32_t ms = load_seg_bytes(t.ms + blk);
     uint32_t out = 0u;
 #pragma unroll
     for (int it = 0; it < kStIter; ++it) {
       uint32_t mb = seg_byte(ms, it);
-      sq = momentum_step8<true>(t, i0 + it * 256, 8, g[it], c[it], mb, a.beta1, e.key, (uint32_t)b, sq);
-      out |= mb << (8 * it);
+      sq = momentum_step8<true>(t, i0 + it * 256, 8, g[it], c[it], mb, a.beta1, rnd, it * 64, sq);
+      out = put_byte(out, mb, it);
     }
-    store_seg_bytes(t.ms + seg / kQBlock, out);
+    store_seg_bytes(t.ms + blk, out);
   } else {
 #pragma unroll 1
     for (int it = 0; it < kStIter && seg + it * 256 < e.run; ++it) {
@@ -632,9 +641,9 @@ __global__ void __launch_bounds__(kStThreads) momentum8_kernel(const __grid_cons
       const int n = (int)max64(0, min64(8, e.run - i));
       Raw8<P> g;
       load_raw<false>(t.g + i, n, g);
-      uint32_t mb = n > 0 ? t.ms[i / kQBlock] : 0u;
-      sq = momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, a.beta1, e.key, (uint32_t)b, sq);
-      if (n > 0 && (threadIdx.x & 15) == 0) t.ms[i / kQBlock] = (uint8_t)mb;
+      uint32_t mb = n > 0 ? t.ms[i >> 7] : 0u;
+      sq = momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, a.beta1, rnd, it * 64, sq);
+      if (n > 0 && (threadIdx.x & 15) == 0) t.ms[i >> 7] = (uint8_t)mb;
     }
   }
   if (e.x != nullptr) {
@@ -692,7 +701,7 @@ __global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __gri
   const StMomentum& e = a.tb.t[ti];
   const int64_t local = blockIdx.x - a.tb.start[ti];
   const int64_t b = local / e.chunks, base = (local - b * e.chunks) * kStChunk;
-  const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8;
+  const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8, blk = seg >> 7;
   const StMatrix<P> t = matrix_of<P>(e, b);
   X* xb = (X*)e.x + b * (e.run / e.cols) * e.ldx;
   const float inv = 1.f / (e.norm[b] + 1e-8f);
@@ -704,7 +713,7 @@ __global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __gri
       load_raw<true>(t.g + i0 + it * 256, 8, g[it]);
       c[it] = load_codes<true>(t.m + i0 + it * 256, 8);
     }
-    const uint32_t ms = load_seg_bytes(t.ms + seg / kQBlock);
+    const uint32_t ms = load_seg_bytes(t.ms + blk);
 #pragma unroll
     for (int it = 0; it < kStIter; ++it)
       input_step8<true>(e, xb, i0 + it * 256, 8, g[it], c[it], seg_byte(ms, it), a.beta1, inv);
@@ -716,7 +725,7 @@ __global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __gri
       if (n == 0) break;
       Raw8<P> g;
       load_raw<false>(t.g + i, n, g);
-      input_step8<false>(e, xb, i, n, g, load_codes<false>(t.m + i, n), t.ms[i / kQBlock], a.beta1, inv);
+      input_step8<false>(e, xb, i, n, g, load_codes<false>(t.m + i, n), t.ms[i >> 7], a.beta1, inv);
     }
   }
 }
