@@ -421,7 +421,8 @@ THORN_API int thorn_adamw_master_multi(const thorn_adamw_state_tensor* tensors, 
  * to 8 bits (the blocks restart at each matrix of the batch);  u = g + beta1 m
  * from the rounded m;  x = u / (||u||_F + 1e-8) per matrix, rounded once to
  * x_dtype (fp16 or bf16), in rows of leading dimension ldx.  x == NULL: the
- * momentum only.  Scratch need not be cleared. */
+ * momentum only.  Tensors of one call need disjoint scratch, which need not be
+ * cleared. */
 typedef struct {
   const void* g;      /* grad (p_dtype), [batch, rows, cols] */
   void* m;            /* e4m3 codes, same shape */
@@ -430,7 +431,7 @@ typedef struct {
   int64_t batch, rows, cols;
   int64_t ldx;        /* >= cols */
   uint64_t seed;
-  void* scratch;      /* with x: thorn_momentum8_scratch_bytes(batch, rows, cols) bytes, 4-byte aligned */
+  void* scratch;      /* with x: thorn_momentum8_scratch_bytes(batch, rows, cols) bytes, 16-byte aligned */
 } thorn_momentum8_tensor;
 
 THORN_API int64_t thorn_momentum8_scratch_bytes(int64_t batch, int64_t rows, int64_t cols);

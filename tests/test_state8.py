@@ -66,22 +66,24 @@ def test_prototypes_match_header():
         m = re.search(r"THORN_API\s+(\w+)\s+" + name + r"\s*\(([^)]*)\)\s*;", text)
         assert scalars[m.group(1)] is res, name
         params = [a.strip().rsplit(None, 1)[0].replace("const", "").strip() for a in m.group(2).split(",")]
-        params = [p + "*" if "*" in a else p for p, a in zip(params, m.group(2).split(","))]
+        params = [p.rstrip("* ") + "*" if "*" in a else p for p, a in zip(params, m.group(2).split(","))]
         assert len(params) == len(argtypes), name
         for decl, got in zip(params, argtypes):
             t = decl.rstrip("* ")
             if t in STRUCTS:
                 assert got is ctypes.POINTER(STRUCTS[t][0]), (name, decl)
-            elif t == "void":
+            elif decl.endswith("*"):
                 assert got is ctypes.c_void_p, (name, decl)
             else:
                 assert got is scalars[decl], (name, decl, got)
 
 
 def test_scratch_bytes(lib):
-    # a norm per matrix and one partial sum per 8192 elements of a matrix, in fp32
-    assert lib.thorn_momentum8_scratch_bytes(1, 64, 128) == (1 + 1) * 4
-    assert lib.thorn_momentum8_scratch_bytes(3, 65, 128) == (3 + 3 * 2) * 4
+    # for matrices longer than 8192 elements: an fp32 sum per 8192 elements and one per matrix,
+    # padded to 16 bytes
+    assert lib.thorn_momentum8_scratch_bytes(7, 64, 128) == 0
+    assert lib.thorn_momentum8_scratch_bytes(3, 65, 128) == 48
+    assert lib.thorn_momentum8_scratch_bytes(5, 128, 128) == 64
     assert lib.thorn_momentum8_scratch_bytes(0, 8, 8) == 0
     assert lib.thorn_momentum8_scratch_bytes(1, 1 << 40, 1 << 40) == 0  # over the size limit
 
@@ -109,7 +111,7 @@ def test_argument_validation_without_gpu(lib):
     assert adam(lib.thorn_adamw_master_multi, w=None) == 1 and adam(lib.thorn_adamw_master_multi, dt=N.F32) == 1
 
     def mom(n=1, dt=N.BF16, xdt=N.F16, **kw):
-        t = N.Momentum8Tensor(P, P, P, P, 1, 4, 4, 4, 0, P)
+        t = N.Momentum8Tensor(P, P, P, P, 1, 4096, 4, 4, 0, P)  # a matrix that needs scratch
         for k, v in kw.items():
             setattr(t, k, v)
         return lib.thorn_momentum8_multi(N.array(N.Momentum8Tensor, [t]), n, dt, xdt, 0.9, None)
@@ -118,7 +120,7 @@ def test_argument_validation_without_gpu(lib):
     assert mom(n=-1) == 1 and mom(dt=9) == 1 and mom(xdt=N.F32) == 1
     for k in ("g", "m", "m_scale", "scratch"):
         assert mom(**{k: None}) == 1, k
-    assert mom(ldx=3) == 1 and mom(batch=-1) == 1
+    assert mom(ldx=3) == 1 and mom(batch=-1) == 1 and mom(scratch=P + 4) == 1
     assert mom(rows=1 << 40, cols=1 << 40) == 1 and mom(batch=1 << 31) == 1
 
     def app(n=1, udt=N.F16, dt=N.BF16, **kw):

@@ -207,21 +207,23 @@ __device__ __forceinline__ uint32_t block_scale(uint32_t top, float& inverse) {
 
 // ---------------------------------------------------------------------------
 // 8 consecutive elements as they lie in memory.  FULL: all 8 are inside the tensor and
-// aligned for vector accesses; otherwise the first n, one by one, zeros behind them.
+// aligned for vector accesses; otherwise `n` says how many are inside, plus kVec where the
+// tensor is aligned, and what is not a whole aligned 8 is read one by one, zeros behind.
 // ---------------------------------------------------------------------------
+constexpr int kVec = 16;
 template <class T>
 struct Raw8 {
   uint4 x[sizeof(T) / 2];
 };
 template <bool FULL, class T>
 __device__ __forceinline__ void load_raw(const T* p, int n, Raw8<T>& r) {
-  if constexpr (FULL) {
+  if (FULL || n == 8 + kVec) {
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.x[i] = reinterpret_cast<const uint4*>(p)[i];
   } else {
     T e[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) e[k] = k < n ? p[k] : from_f<T>(0.f);
+    for (int k = 0; k < 8; ++k) e[k] = k < (n & 15) ? p[k] : from_f<T>(0.f);
     memcpy(&r, e, sizeof(r));
   }
 }
@@ -248,28 +250,32 @@ __device__ __forceinline__ void store8(T* p, const f2* v, int n) {
     float x[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) unpack_f2(v[k], x[2 * k], x[2 * k + 1]);
-    store_n(p, x, FULL ? 8 : n, FULL);
+    store_n(p, x, FULL ? 8 : n & 15, FULL || (n & kVec));
   }
 }
 template <bool FULL>
 __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int n) {
-  if constexpr (FULL) return *reinterpret_cast<const uint2*>(p);
+  if (FULL || n == 8 + kVec) return *reinterpret_cast<const uint2*>(p);
   uint32_t w[2] = {0u, 0u};
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    if (k < n) w[k >> 2] |= (uint32_t)p[k] << (8 * (k & 3));
+    if (k < (n & 15)) w[k >> 2] |= (uint32_t)p[k] << (8 * (k & 3));
   return make_uint2(w[0], w[1]);
 }
 template <bool FULL>
 __device__ __forceinline__ void store_codes(uint8_t* p, uint2 c, int n) {
-  if constexpr (FULL) {
+  if (FULL || n == 8 + kVec) {
     *reinterpret_cast<uint2*>(p) = c;
   } else {
     const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (k < n) p[k] = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
+      if (k < (n & 15)) p[k] = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
   }
+}
+
+__device__ __forceinline__ int elems8(int64_t i, int64_t end, int vec) {
+  return (int)max64(0, min64(8, end - i)) + (vec ? kVec : 0);
 }
 
 // A warp's segment of a chunk is kStSeg consecutive elements, taken 256 at a time: 8 blocks
@@ -490,9 +496,14 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
 }
 
 // S8: moments in 8 bits, else fp32.  MASTER: the update is applied to fp32 master weights
-// and p receives their rounding.
+// and p receives their rounding.  The 8-bit form
+// without masters at four blocks per SM (64 registers): 1749 us for two 128256 x 4096
+// tensors, 1808 at the registers that it takes by itself, 1965 at three blocks and 1766 at
+// five, which spill.  The forms that move more bytes per element at three (80 registers): at
+// the 86 that it takes by itself 151936 x 1024 with masters took 450 us instead of 389.
 template <class P, bool S8, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kStThreads) adamw_state_kernel(const __grid_constant__ StAdamArgs<CAP> a) {
+__global__ void __launch_bounds__(kStThreads, S8 && !MASTER ? 4 : 3)
+    adamw_state_kernel(const __grid_constant__ StAdamArgs<CAP> a) {
   const int ti = st_find(a.tb, blockIdx.x);
   const StAdam& e = a.tb.t[ti];
   const int64_t base = int64_t(blockIdx.x - a.tb.start[ti]) * kStChunk;
@@ -526,16 +537,17 @@ __global__ void __launch_bounds__(kStThreads) adamw_state_kernel(const __grid_co
 #pragma unroll 1
     for (int it = 0; it < kStIter && seg + it * 256 < e.numel; ++it) {
       const int64_t i = i0 + it * 256;
-      const int n = (int)max64(0, min64(8, e.numel - i));
+      const int n = elems8(i, e.numel, e.vec);
+      const bool some = i < e.numel;
       In in;
       adam_load<false>(e, i, n, in);
       uint32_t mb = 0u, vb = 0u;
-      if (S8 && n > 0) {
+      if (S8 && some) {
         mb = e.ms[i >> 7];
         vb = e.vs[i >> 7];
       }
       adam_step8<false>(e, a.s, i, n, in, rnd, it * 64, mb, vb);
-      if (S8 && n > 0 && (threadIdx.x & 15) == 0) {
+      if (S8 && some && (threadIdx.x & 15) == 0) {
         e.ms[i >> 7] = (uint8_t)mb;
         e.vs[i >> 7] = (uint8_t)vb;
       }
@@ -546,15 +558,21 @@ __global__ void __launch_bounds__(kStThreads) adamw_state_kernel(const __grid_co
 // ===========================================================================
 // momentum in 8 bits and the Newton-Schulz input
 // ===========================================================================
+// Matrices of one tensor, as one launch sees them.  Three forms by the matrix's length: up to
+// kStSeg elements a warp holds a whole matrix, up to kStChunk a block does; both then write
+// the input from registers.  Longer matrices take two readings: the momentum leaves one partial
+// sum of squares per chunk, and the input reads g and the new codes again.
 struct StMomentum {
   const void* g;
   uint8_t* m;
   uint8_t* ms;
   void* x;
-  float* norm;   // [batch], then [batch][chunks] partial sums of squares
-  int64_t batch, cols, ldx;
+  float* part;   // [matrices][chunks] partial sums of squares
+  float* norm;   // [matrices] their sums, where a launch of its own forms them
   int64_t run;   // elements of one matrix
-  int64_t chunks;
+  int64_t cols, ldx;
+  int64_t batch;
+  int64_t chunks;        // of one matrix
   uint64_t key;
   int vec;
 };
@@ -576,11 +594,11 @@ __device__ __forceinline__ StMatrix<P> matrix_of(const StMomentum& e, int64_t b)
   return StMatrix<P>{(const P*)e.g + b * e.run, e.m + b * e.run, e.ms + b * ((e.run + kQBlock - 1) / kQBlock)};
 }
 
-// Momentum of one thread's 8 elements, mb as above; adds the squares of u = g + beta1 m.
+// Momentum of one thread's 8 elements, mb as above; u = g + beta1 m from the rounded m.
 template <bool FULL, class P>
-__device__ __forceinline__ f2 momentum_step8(const StMatrix<P>& t, int64_t i0, int n, const Raw8<P>& graw, uint2 c,
-                                             uint32_t& mb, float beta1, const Rounding& rnd, uint32_t step, f2 sq) {
-  f2 g[4], m[4], y[4];
+__device__ __forceinline__ void momentum_step8(const StMatrix<P>& t, int64_t i0, int n, const Raw8<P>& graw, uint2 c,
+                                               uint32_t& mb, float beta1, const Rounding& rnd, uint32_t step, f2* u) {
+  f2 g[4], m[4];
   values(graw, g);
   decode8(c, m);
   const f2 s = dup(scale_value(mb) * beta1);
@@ -593,30 +611,48 @@ __device__ __forceinline__ f2 momentum_step8(const StMatrix<P>& t, int64_t i0, i
   mb = block_scale(top, inv1);
   const f2 inv = dup(inv1);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) y[k] = mul(m[k], inv);
-  c = encode8(y, rnd.bits(step), rnd.bits(step + 1));
+  for (int k = 0; k < 4; ++k) m[k] = mul(m[k], inv);
+  c = encode8(m, rnd.bits(step), rnd.bits(step + 1));
   store_codes<FULL>(t.m + i0, c, n);
   decode8(c, m);
   const f2 s2 = dup(scale_value(mb) * beta1);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const f2 u = add(g[k], mul(m[k], s2));
-    sq = fma(u, u, sq);
-  }
-  return sq;
+  for (int k = 0; k < 4; ++k) u[k] = add(g[k], mul(m[k], s2));
 }
 
-template <class P, int CAP>
-__global__ void __launch_bounds__(kStThreads) momentum8_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
-  __shared__ float red[32];
-  const int ti = st_find(a.tb, blockIdx.x);
-  const StMomentum& e = a.tb.t[ti];
-  const int64_t local = blockIdx.x - a.tb.start[ti];
-  const int64_t b = local / e.chunks, base = (local - b * e.chunks) * kStChunk;
+// x = u * inv of 8 elements of a matrix
+template <bool FULL, class X>
+__device__ __forceinline__ void store_input8(const StMomentum& e, X* xb, int64_t i0, int n, f2* u, float inv1) {
+  const f2 inv = dup(inv1);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) u[k] = mul(u[k], inv);
+  if (FULL || e.ldx == e.cols) {
+    store8<FULL>(xb + i0, u, n);
+  } else {  // rows padded to a longer leading dimension
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) unpack_f2(u[k], v[2 * k], v[2 * k + 1]);
+    int64_t r = i0 / e.cols, col = i0 - r * e.cols;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k < (n & 15)) xb[r * e.ldx + col] = from_f<X>(v[k]);
+      if (++col == e.cols) {
+        col = 0;
+        ++r;
+      }
+    }
+  }
+}
+__device__ __forceinline__ float inverse_norm(float sumsq) { return 1.f / (sqrtf(sumsq) + 1e-8f); }
+
+// Momentum of one chunk by the block; returns this thread's sum of squares of u.
+template <class P>
+__device__ __forceinline__ float momentum_chunk(const StMomentum& e, float beta1, int64_t b, int64_t chunk) {
+  const int64_t base = chunk * kStChunk;
   const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8, blk = seg >> 7;
   const StMatrix<P> t = matrix_of<P>(e, b);
   const Rounding rnd(i0, e.key, (uint32_t)b);
-  f2 sq = dup(0.f);
+  f2 sq = dup(0.f), u[4];
   if (e.vec && base + kStChunk <= e.run) {
     Raw8<P> g[kStIter];
     uint2 c[kStIter];
@@ -630,7 +666,9 @@ __global__ void __launch_bounds__(kStThreads) momentum8_kernel(const __grid_cons
 #pragma unroll
     for (int it = 0; it < kStIter; ++it) {
       uint32_t mb = seg_byte(ms, it);
-      sq = momentum_step8<true>(t, i0 + it * 256, 8, g[it], c[it], mb, a.beta1, rnd, it * 64, sq);
+      momentum_step8<true>(t, i0 + it * 256, 8, g[it], c[it], mb, beta1, rnd, it * 64, u);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sq = fma(u[k], u[k], sq);
       out = put_byte(out, mb, it);
     }
     store_seg_bytes(t.ms + blk, out);
@@ -638,94 +676,149 @@ __global__ void __launch_bounds__(kStThreads) momentum8_kernel(const __grid_cons
 #pragma unroll 1
     for (int it = 0; it < kStIter && seg + it * 256 < e.run; ++it) {
       const int64_t i = i0 + it * 256;
-      const int n = (int)max64(0, min64(8, e.run - i));
+      const int n = elems8(i, e.run, e.vec);
       Raw8<P> g;
       load_raw<false>(t.g + i, n, g);
-      uint32_t mb = n > 0 ? t.ms[i >> 7] : 0u;
-      sq = momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, a.beta1, rnd, it * 64, sq);
-      if (n > 0 && (threadIdx.x & 15) == 0) t.ms[i >> 7] = (uint8_t)mb;
+      uint32_t mb = i < e.run ? t.ms[i >> 7] : 0u;
+      momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, beta1, rnd, it * 64, u);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sq = fma(u[k], u[k], sq);
+      if (i < e.run && (threadIdx.x & 15) == 0) t.ms[i >> 7] = (uint8_t)mb;
     }
   }
-  if (e.x != nullptr) {
-    float s0, s1;
-    unpack_f2(sq, s0, s1);
-    const float tot = block_sum(s0 + s1, red);
-    if (threadIdx.x == 0) e.norm[e.batch + local] = tot;
-  }
+  float s0, s1;
+  unpack_f2(sq, s0, s1);
+  return s0 + s1;
 }
 
-// One block per matrix: the fixed-order sum of its chunks' partials, and its root.
-template <int CAP>
-__global__ void __launch_bounds__(kStThreads) momentum8_norm_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
-  __shared__ double red[32];
-  const int ti = st_find(a.tb, blockIdx.x);
-  const StMomentum& e = a.tb.t[ti];
-  const int64_t b = blockIdx.x - a.tb.start[ti];
-  const float* part = e.norm + e.batch + b * e.chunks;
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < e.chunks; i += kStThreads) s += (double)part[i];
-  s = block_sum_d(s, red);
-  if (threadIdx.x == 0) e.norm[b] = sqrtf((float)s);
-}
-
-template <bool FULL, class P, class X>
-__device__ __forceinline__ void input_step8(const StMomentum& e, X* xb, int64_t i0, int n, const Raw8<P>& graw, uint2 c,
-                                            uint32_t mb, float beta1, float inv1) {
-  f2 g[4], m[4];
-  values(graw, g);
-  decode8(c, m);
-  const f2 s = dup(scale_value(mb) * beta1), inv = dup(inv1);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) m[k] = mul(add(g[k], mul(m[k], s)), inv);
-  if (FULL || e.ldx == e.cols) {
-    store8<FULL>(xb + i0, m, n);
-  } else {  // rows padded to a longer leading dimension
-    float u[8];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) unpack_f2(m[k], u[2 * k], u[2 * k + 1]);
-    int64_t r = i0 / e.cols, col = i0 - r * e.cols;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (k < n) xb[r * e.ldx + col] = from_f<X>(u[k]);
-      if (++col == e.cols) {
-        col = 0;
-        ++r;
-      }
-    }
-  }
-}
-
-template <class P, class X, int CAP>
-__global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
+// The momentum pass.  Six blocks per SM (40 registers): more loads in flight than at the
+// registers that it takes by itself (decoder layer of 218 M elements, both passes: 322 us
+// against 339).
+template <class P, int CAP>
+__global__ void __launch_bounds__(kStThreads, 6) momentum8_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
+  __shared__ float red[32];
   const int ti = st_find(a.tb, blockIdx.x);
   const StMomentum& e = a.tb.t[ti];
   const int64_t local = blockIdx.x - a.tb.start[ti];
+  const int64_t b = local / e.chunks;
+  const float sq = momentum_chunk<P>(e, a.beta1, b, local - b * e.chunks);
+  if (e.x != nullptr) {
+    const float tot = block_sum(sq, red);
+    if (threadIdx.x == 0) e.part[local] = tot;
+  }
+}
+
+// Matrices that a warp (WARP) or a block holds: momentum, norm and input at once.
+template <class P, class X, bool WARP, int CAP>
+__global__ void __launch_bounds__(kStThreads) momentum8_small_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
+  __shared__ float red[32];
+  const int ti = st_find(a.tb, blockIdx.x);
+  const StMomentum& e = a.tb.t[ti];
+  const int64_t local = blockIdx.x - a.tb.start[ti];
+  const int warp = threadIdx.x >> 5;
+  const int64_t b = WARP ? local * (kStThreads / 32) + warp : local;
+  if (WARP && b >= e.batch) return;  // whole warps, and no block-wide step in this form
+  const int64_t seg = WARP ? 0 : warp * kStSeg, i0 = seg + (threadIdx.x & 31) * 8;
+  const StMatrix<P> t = matrix_of<P>(e, b);
+  const Rounding rnd(i0, e.key, (uint32_t)b);
+  f2 sq = dup(0.f), u[kStIter][4];
+#pragma unroll
+  for (int it = 0; it < kStIter; ++it) {
+    if (seg + it * 256 >= e.run) break;
+    const int64_t i = i0 + it * 256;
+    const int n = elems8(i, e.run, e.vec);
+    Raw8<P> g;
+    load_raw<false>(t.g + i, n, g);
+    uint32_t mb = i < e.run ? t.ms[i >> 7] : 0u;
+    momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, a.beta1, rnd, it * 64, u[it]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sq = fma(u[it][k], u[it][k], sq);
+    if (i < e.run && (threadIdx.x & 15) == 0) t.ms[i >> 7] = (uint8_t)mb;
+  }
+  float s0, s1;
+  unpack_f2(sq, s0, s1);
+  const float inv = inverse_norm(WARP ? warp_sum(s0 + s1) : block_sum(s0 + s1, red));
+  X* xb = (X*)e.x + b * (e.run / e.cols) * e.ldx;
+#pragma unroll
+  for (int it = 0; it < kStIter; ++it) {
+    const int64_t i = i0 + it * 256;
+    if (i >= e.run) break;
+    store_input8<false>(e, xb, i, elems8(i, e.run, e.vec), u[it], inv);
+  }
+}
+
+// Partials that an input block sums by itself; the norm of a longer matrix is formed once,
+// by a launch between the passes.
+constexpr int kOwnSum = kStThreads;
+
+template <int CAP>
+__global__ void __launch_bounds__(1024) momentum8_norm_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
+  __shared__ float red[32];
+  const int ti = st_find(a.tb, blockIdx.x);
+  const StMomentum& e = a.tb.t[ti];
+  const int64_t b = blockIdx.x - a.tb.start[ti];
+  const float* part = e.part + b * e.chunks;
+  float s = 0.f;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < e.chunks; i += 1024) s += part[i];
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) e.norm[b] = s;
+}
+
+// The input pass, from the last chunk to the first: what the momentum pass read and wrote
+// last is then still in L2.
+template <class P, class X, int CAP>
+__global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
+  __shared__ float red[32];
+  const uint32_t bid = gridDim.x - 1 - blockIdx.x;
+  const int ti = st_find(a.tb, bid);
+  const StMomentum& e = a.tb.t[ti];
+  const int64_t local = bid - a.tb.start[ti];
   const int64_t b = local / e.chunks, base = (local - b * e.chunks) * kStChunk;
   const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8, blk = seg >> 7;
   const StMatrix<P> t = matrix_of<P>(e, b);
   X* xb = (X*)e.x + b * (e.run / e.cols) * e.ldx;
-  const float inv = 1.f / (e.norm[b] + 1e-8f);
-  if (e.vec && e.ldx == e.cols && base + kStChunk <= e.run) {
-    Raw8<P> g[kStIter];
-    uint2 c[kStIter];
+  const bool full = e.vec && e.ldx == e.cols && base + kStChunk <= e.run;
+  Raw8<P> g[kStIter];
+  uint2 c[kStIter];
+  uint32_t ms = 0u;
+  if (full) {
 #pragma unroll
     for (int it = 0; it < kStIter; ++it) {
       load_raw<true>(t.g + i0 + it * 256, 8, g[it]);
       c[it] = load_codes<true>(t.m + i0 + it * 256, 8);
     }
-    const uint32_t ms = load_seg_bytes(t.ms + blk);
+    ms = load_seg_bytes(t.ms + blk);
+  }
+  float sumsq;
+  if (e.chunks <= kOwnSum) sumsq = block_sum(threadIdx.x < e.chunks ? e.part[b * e.chunks + threadIdx.x] : 0.f, red);
+  else sumsq = e.norm[b];
+  const float inv = inverse_norm(sumsq);
+  f2 u[4], q[4];
+  if (full) {
 #pragma unroll
-    for (int it = 0; it < kStIter; ++it)
-      input_step8<true>(e, xb, i0 + it * 256, 8, g[it], c[it], seg_byte(ms, it), a.beta1, inv);
+    for (int it = 0; it < kStIter; ++it) {
+      values(g[it], q);
+      decode8(c[it], u);
+      const f2 s = dup(scale_value(seg_byte(ms, it)) * a.beta1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = add(q[k], mul(u[k], s));
+      store_input8<true>(e, xb, i0 + it * 256, 8, u, inv);
+    }
   } else {
 #pragma unroll 1
     for (int it = 0; it < kStIter; ++it) {
       const int64_t i = i0 + it * 256;
-      const int n = (int)max64(0, min64(8, e.run - i));
-      if (n == 0) break;
-      Raw8<P> g;
-      load_raw<false>(t.g + i, n, g);
-      input_step8<false>(e, xb, i, n, g, load_codes<false>(t.m + i, n), t.ms[i >> 7], a.beta1, inv);
+      if (i >= e.run) break;
+      const int n = elems8(i, e.run, e.vec);
+      Raw8<P> r;
+      load_raw<false>(t.g + i, n, r);
+      values(r, q);
+      decode8(load_codes<false>(t.m + i, n), u);
+      const f2 s = dup(scale_value(t.ms[i >> 7]) * a.beta1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) u[k] = add(q[k], mul(u[k], s));
+      store_input8<false>(e, xb, i, n, u, inv);
     }
   }
 }
@@ -770,7 +863,7 @@ __device__ __forceinline__ void apply_step8(const StApply& e, float wd, int64_t 
     int64_t r = i0 / e.cols, c = i0 - r * e.cols;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (FULL || k < n) {
+      if (FULL || k < (n & 15)) {
         float s = e.row_scale[r];
         if (e.mat_stats != nullptr) {
           const int64_t b = r / e.rows;
@@ -808,8 +901,8 @@ __global__ void __launch_bounds__(kStThreads) apply_master_kernel(const __grid_c
 #pragma unroll 1
     for (int it = 0; it < kStChunk / kStStep; ++it) {
       const int64_t i0 = base + it * kStStep + threadIdx.x * 8;
-      const int n = (int)max64(0, min64(8, e.numel - i0));
-      if (n == 0) break;
+      if (i0 >= e.numel) break;
+      const int n = elems8(i0, e.numel, e.vec);
       apply_step8<U, P, false>(e, a.wd, i0, n);
     }
   }
@@ -819,6 +912,7 @@ __global__ void __launch_bounds__(kStThreads) apply_master_kernel(const __grid_c
 // dispatch
 // ---------------------------------------------------------------------------
 constexpr int kStCap = 32;  // tensors per launch
+
 
 static bool st_half(int d) { return d == THORN_BF16 || d == THORN_F16; }
 static bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
@@ -896,8 +990,90 @@ extern "C" int thorn_adamw_master_multi(const thorn_adamw_state_tensor* ts, int 
 }
 
 extern "C" int64_t thorn_momentum8_scratch_bytes(int64_t batch, int64_t rows, int64_t cols) {
-  if (st_elems(batch, rows, cols) <= 0) return 0;
-  return (batch + batch * st_cdiv(rows * cols, kStChunk)) * (int64_t)sizeof(float);
+  if (st_elems(batch, rows, cols) <= 0 || rows * cols <= kStChunk) return 0;
+  return st_cdiv(batch * (st_cdiv(rows * cols, kStChunk) + 1), 4) * 16;
+}
+
+template <class P, class X>
+static int momentum_launch(const thorn_momentum8_tensor* ts, int n, float beta1, cudaStream_t st) {
+  using Table = StTable<StMomentum, kStCap>;
+  auto args = [&](const Table& tb) {
+    StMomentumArgs<kStCap> a;
+    a.tb = tb;
+    a.beta1 = beta1;
+    return a;
+  };
+  auto entry = [](const thorn_momentum8_tensor& t) {
+    const int64_t run = t.rows * t.cols;
+    StMomentum e{};
+    e.g = t.g;
+    e.m = (uint8_t*)t.m;
+    e.ms = (uint8_t*)t.m_scale;
+    e.x = t.x;
+    e.run = run;
+    e.cols = t.cols;
+    e.ldx = t.ldx;
+    e.batch = t.batch;
+    e.chunks = st_cdiv(run, kStChunk);
+    e.key = rounding_key(t.seed);
+    e.vec = (t.batch == 1 || run % 8 == 0) && aligned16(t.g) && aligned8(t.m) && aligned16(t.x);
+    if (t.x && run > kStChunk) {
+      e.norm = (float*)t.scratch;
+      e.part = e.norm + t.batch;
+    }
+    return e;
+  };
+  auto live = [](const thorn_momentum8_tensor& t) { return st_elems(t.batch, t.rows, t.cols) > 0; };
+  int rc = st_launch<StMomentum, kStCap>(
+      ts, n,
+      [&](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t {
+        if (!live(t) || !t.x || t.rows * t.cols > kStSeg) return 0;
+        e = entry(t);
+        return st_cdiv(t.batch, kStThreads / 32);
+      },
+      [&](const Table& tb, unsigned nb) {
+        momentum8_small_kernel<P, X, true, kStCap><<<nb, kStThreads, 0, st>>>(args(tb));
+      });
+  if (rc) return rc;
+  rc = st_launch<StMomentum, kStCap>(
+      ts, n,
+      [&](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t {
+        if (!live(t) || !t.x || t.rows * t.cols <= kStSeg || t.rows * t.cols > kStChunk) return 0;
+        e = entry(t);
+        return t.batch;
+      },
+      [&](const Table& tb, unsigned nb) {
+        momentum8_small_kernel<P, X, false, kStCap><<<nb, kStThreads, 0, st>>>(args(tb));
+      });
+  if (rc) return rc;
+  // momentum only, or longer than a block holds
+  auto is_long = [&](const thorn_momentum8_tensor& t) { return live(t) && (!t.x || t.rows * t.cols > kStChunk); };
+  rc = st_launch<StMomentum, kStCap>(
+      ts, n,
+      [&](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t {
+        if (!is_long(t)) return 0;
+        e = entry(t);
+        return t.batch * e.chunks;
+      },
+      [&](const Table& tb, unsigned nb) { momentum8_kernel<P, kStCap><<<nb, kStThreads, 0, st>>>(args(tb)); });
+  if (rc) return rc;
+  rc = st_launch<StMomentum, kStCap>(
+      ts, n,
+      [&](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t {
+        if (!is_long(t) || !t.x) return 0;
+        e = entry(t);
+        return e.chunks > kOwnSum ? t.batch : 0;
+      },
+      [&](const Table& tb, unsigned nb) { momentum8_norm_kernel<kStCap><<<nb, 1024, 0, st>>>(args(tb)); });
+  if (rc) return rc;
+  return st_launch<StMomentum, kStCap>(
+      ts, n,
+      [&](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t {
+        if (!is_long(t) || !t.x) return 0;
+        e = entry(t);
+        return t.batch * e.chunks;
+      },
+      [&](const Table& tb, unsigned nb) { momentum8_input_kernel<P, X, kStCap><<<nb, kStThreads, 0, st>>>(args(tb)); });
 }
 
 extern "C" int thorn_momentum8_multi(const thorn_momentum8_tensor* ts, int n, int p_dtype, int x_dtype, float beta1,
@@ -909,48 +1085,20 @@ extern "C" int thorn_momentum8_multi(const thorn_momentum8_tensor* ts, int n, in
     const int64_t k = st_elems(t.batch, t.rows, t.cols);
     if (k < 0) return THORN_ERR_ARG;
     if (k == 0) continue;
-    if (!t.g || !t.m || !t.m_scale || (t.x && (!t.scratch || t.ldx < t.cols || t.ldx > kStMaxElems / (t.batch * t.rows))))
-      return THORN_ERR_ARG;
-    if (t.batch > kStMaxGrid || t.batch > kStMaxGrid / st_cdiv(t.rows * t.cols, kStChunk)) return THORN_ERR_ARG;
+    if (!t.g || !t.m || !t.m_scale) return THORN_ERR_ARG;
+    if (t.x && (t.ldx < t.cols || t.ldx > kStMaxElems / (t.batch * t.rows))) return THORN_ERR_ARG;
+    if (t.x && t.rows * t.cols > kStChunk && (!t.scratch || !aligned16(t.scratch))) return THORN_ERR_ARG;
+    if (t.batch > kStMaxGrid / st_cdiv(t.rows * t.cols, kStChunk)) return THORN_ERR_ARG;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  auto entry = [](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t {
-    if (st_elems(t.batch, t.rows, t.cols) <= 0) return 0;
-    const int64_t run = t.rows * t.cols;
-    e = StMomentum{t.g, (uint8_t*)t.m, (uint8_t*)t.m_scale, t.x, (float*)t.scratch, t.batch, t.cols, t.ldx, run,
-                   st_cdiv(run, kStChunk), rounding_key(t.seed), 0};
-    e.vec = (t.batch == 1 || run % 8 == 0) && aligned16(t.g) && aligned8(t.m) && aligned16(t.x);
-    return t.batch * e.chunks;
-  };
-  auto with_x = [&](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t { return t.x ? entry(t, e) : 0; };
-  auto each_p = [&](auto f) -> int {
-    if (p_dtype == THORN_F32) return f((float*)nullptr);
-    if (p_dtype == THORN_BF16) return f((__nv_bfloat16*)nullptr);
-    return f((__half*)nullptr);
-  };
-  auto args = [&](const StTable<StMomentum, kStCap>& tb) {
-    StMomentumArgs<kStCap> a;
-    a.tb = tb;
-    a.beta1 = beta1;
-    return a;
-  };
-  return each_p([&](auto* pp) -> int {
+  auto with_p = [&](auto* pp) -> int {
     using P = std::remove_pointer_t<decltype(pp)>;
-    int rc = st_launch<StMomentum, kStCap>(ts, n, entry, [&](const StTable<StMomentum, kStCap>& tb, unsigned nb) {
-      momentum8_kernel<P, kStCap><<<nb, kStThreads, 0, st>>>(args(tb));
-    });
-    if (rc) return rc;
-    rc = st_launch<StMomentum, kStCap>(
-        ts, n, [&](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t { return with_x(t, e) > 0 ? t.batch : 0; },
-        [&](const StTable<StMomentum, kStCap>& tb, unsigned nb) {
-          momentum8_norm_kernel<kStCap><<<nb, kStThreads, 0, st>>>(args(tb));
-        });
-    if (rc) return rc;
-    return st_launch<StMomentum, kStCap>(ts, n, with_x, [&](const StTable<StMomentum, kStCap>& tb, unsigned nb) {
-      if (x_dtype == THORN_F16) momentum8_input_kernel<P, __half, kStCap><<<nb, kStThreads, 0, st>>>(args(tb));
-      else momentum8_input_kernel<P, __nv_bfloat16, kStCap><<<nb, kStThreads, 0, st>>>(args(tb));
-    });
-  });
+    if (x_dtype == THORN_F16) return momentum_launch<P, __half>(ts, n, beta1, st);
+    return momentum_launch<P, __nv_bfloat16>(ts, n, beta1, st);
+  };
+  if (p_dtype == THORN_F32) return with_p((float*)nullptr);
+  if (p_dtype == THORN_BF16) return with_p((__nv_bfloat16*)nullptr);
+  return with_p((__half*)nullptr);
 }
 
 extern "C" int thorn_apply_master_multi(const thorn_apply_master_tensor* ts, int n, int u_dtype, int p_dtype,

@@ -25,7 +25,10 @@ the parameter's dtype (thorn.py:1591-1599) and updates 16-bit parameters in plac
 from __future__ import annotations
 
 import struct
+from functools import lru_cache
+from itertools import repeat
 from math import prod
+from operator import attrgetter
 from typing import Optional, Sequence, Union
 
 import torch
@@ -69,20 +72,33 @@ def _lists(**named):
     return list(out.values())
 
 
-def _check(ts, dtype, dev, what, shapes=None, distinct=True):
-    for i, t in enumerate(ts):
-        if t.dtype is not dtype:
-            raise TypeError(f"{what}[{i}] must be {dtype}, got {t.dtype}")
-        if t.device != dev:
-            raise RuntimeError(f"{what}[{i}] is on {t.device}, expected {dev}")
-        if not t.is_contiguous():
-            raise ValueError(f"{what}[{i}] must be contiguous")
-        if shapes is not None and t.shape != shapes[i]:
-            raise ValueError(f"{what}[{i}] must have shape {tuple(shapes[i])}, got {tuple(t.shape)}")
-    if distinct:
-        ptrs = [t.data_ptr() for t in ts if t.numel()]
-        if len(set(ptrs)) != len(ptrs):
+def _check(ts, dtype, dev, what, shapes=None, distinct=True) -> list:
+    """Data pointers of ``ts`` after checking them (whole-list comparisons: a call may bring
+    hundreds of tensors, and the checks are most of its host time)."""
+    index = dev.index if dev.index is not None else -1  # -1: the CPU
+    if not (set(map(_dtype_of, ts)) == {dtype} and set(map(_device_index, ts)) == {index} and all(map(_contiguous, ts))
+            and (shapes is None or list(map(_shape_of, ts)) == shapes)):
+        for i, t in enumerate(ts):
+            if t.dtype is not dtype:
+                raise TypeError(f"{what}[{i}] must be {dtype}, got {t.dtype}")
+            if t.device != dev:
+                raise RuntimeError(f"{what}[{i}] is on {t.device}, expected {dev}")
+            if not t.is_contiguous():
+                raise ValueError(f"{what}[{i}] must be contiguous")
+            if shapes is not None and t.shape != shapes[i]:
+                raise ValueError(f"{what}[{i}] must have shape {tuple(shapes[i])}, got {tuple(t.shape)}")
+        raise RuntimeError(f"{what}: unsupported tensors")
+    ptrs = list(map(_pointer, ts))
+    if distinct and len(set(ptrs)) != len(ptrs):
+        seen = [p for p, t in zip(ptrs, ts) if t.numel()]  # empty tensors may share an address
+        if len(set(seen)) != len(seen):
             raise ValueError(f"{what}: the same tensor is given twice")
+    return ptrs
+
+
+_dtype_of, _shape_of = attrgetter("dtype"), attrgetter("shape")
+_device_index, _contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
+_pointer, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
 
 
 def _device(t) -> torch.device:
@@ -92,6 +108,20 @@ def _device(t) -> torch.device:
         raise RuntimeError("this call takes host scalars (step, learning rate, seeds) that a captured CUDA graph would "
                            "repeat at every replay: call it outside of graph capture")
     return t.device
+
+
+def _strides(shape) -> tuple:
+    """Strides of a contiguous tensor."""
+    out, k = [1], 1
+    for d in reversed(shape[1:]):
+        k *= max(1, d)
+        out.append(k)
+    return tuple(reversed(out))
+
+
+@lru_cache(maxsize=4096)
+def _momentum_scratch(B: int, R: int, C: int) -> int:
+    return int(N.load().thorn_momentum8_scratch_bytes(B, R, C))
 
 
 def _blocks(numel: int) -> int:
@@ -124,15 +154,14 @@ def launch_adam(records, p_dtype, eight: bool, betas, weight_decay: float, eps: 
 
 def launch_momentum8(items, p_dtype, x_dtype, beta: float, dev, stream) -> None:
     """``items``: (g, m, m_scale, x pointer or 0, batch, rows, cols, ldx, seed)."""
-    lib = N.load()
-    need = [lib.thorn_momentum8_scratch_bytes(B, R, C) if x else 0 for _, _, _, x, B, R, C, _, _ in items]
-    scratch = torch.empty(max(4, sum(need)), dtype=torch.uint8, device=dev)
+    need = [_momentum_scratch(B, R, C) if x else 0 for _, _, _, x, B, R, C, _, _ in items]
+    scratch = torch.empty(max(16, sum(need)), dtype=torch.uint8, device=dev)
     recs, at = [], scratch.data_ptr()
     for (g, m, ms, x, B, R, C, ldx, seed), nb in zip(items, need):
         recs.append(_MOMENTUM.pack(g, m, ms, x, B, R, C, ldx, seed & _U64, at if nb else 0))
         at += nb
-    N.check(lib.thorn_momentum8_multi(_records(N.Momentum8Tensor, recs), len(recs), N.dtype_code(p_dtype),
-                                      N.dtype_code(x_dtype), beta, stream), "momentum8_multi")
+    N.check(N.load().thorn_momentum8_multi(_records(N.Momentum8Tensor, recs), len(recs), N.dtype_code(p_dtype),
+                                           N.dtype_code(x_dtype), beta, stream), "momentum8_multi")
 
 
 def launch_apply(items, u_dtype, p_dtype, weight_decay: float, stream) -> None:
@@ -177,49 +206,44 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
         raise ValueError(f"betas must be in [0, 1), got {tuple(betas)}")
-    shapes = [p.shape for p in params]
-    _check(params, pdt, dev, "params")
-    _check(grads, pdt, dev, "grads", shapes, distinct=False)
-    _check(moments, sdt, dev, "moments", shapes)
-    _check(variances, sdt, dev, "variances", shapes)
+    shapes = list(map(_shape_of, params))
+    pp = _check(params, pdt, dev, "params")
+    gp = _check(grads, pdt, dev, "grads", shapes, distinct=False)
+    mp = _check(moments, sdt, dev, "moments", shapes)
+    vp = _check(variances, sdt, dev, "variances", shapes)
+    numels = list(map(_numel, params))
+    wp = msp = vsp = repeat(0)
     if masters is not None:
         if pdt not in _HALF:
             raise TypeError(f"masters are fp32 copies of 16-bit parameters, got {pdt} parameters")
-        _check(masters, torch.float32, dev, "masters", shapes)
+        wp = _check(masters, torch.float32, dev, "masters", shapes)
     if eight:
         if ms is None or vs is None or seeds is None:
             raise ValueError("8-bit moments need moment_scales, variance_scales and seeds")
-        nblk = [(_blocks(p.numel()),) for p in params]
-        _check(ms, SCALES, dev, "moment_scales", nblk)
-        _check(vs, SCALES, dev, "variance_scales", nblk)
-        seeds = _per_tensor(seeds, n, "seeds")
+        blocks = [(-(-k // BLOCK),) for k in numels]
+        msp = _check(ms, SCALES, dev, "moment_scales", blocks)
+        vsp = _check(vs, SCALES, dev, "variance_scales", blocks)
+        seeds = [x & _U64 for x in _per_tensor(seeds, n, "seeds")]
     else:
         if ms is not None or vs is not None:
             raise ValueError(f"scales are given with {sdt} moments")
         N.dtype_code(sdt)
         if masters is not None and sdt is not torch.float32:
             raise TypeError(f"masters need fp32 or 8-bit moments, got {sdt}")
+        seeds = repeat(0)
     scal = {}
-    for s in set(steps):
-        rect = radam_rect(b2, s, rectify)
-        scal[s] = (rect, 1 / (1 - b1 ** s), 1 / (1 - b2 ** s), 1 if rect == 0.0 else 0)
-    recs = []
-    for i in range(n):
-        p = params[i]
-        rect, bc1, bc2, deg = scal[steps[i]]
-        if eight or masters is not None:
-            recs.append(adam_record(p.data_ptr(), grads[i].data_ptr(), 0 if masters is None else masters[i].data_ptr(),
-                                    moments[i].data_ptr(), variances[i].data_ptr(), ms[i].data_ptr() if eight else 0,
-                                    vs[i].data_ptr() if eight else 0, p.numel(), seeds[i] if eight else 0,
-                                    lrs[i] * rect, bc1, bc2, deg))
-        else:
-            recs.append(N.AdamTensor(p.data_ptr(), grads[i].data_ptr(), moments[i].data_ptr(),
-                                     variances[i].data_ptr(), p.numel(), lrs[i] * rect, bc1, bc2, deg))
+    for t in set(steps):
+        scal[t] = (radam_rect(b2, t, rectify), 1 / (1 - b1 ** t), 1 / (1 - b2 ** t))
+    rects, bc1, bc2 = zip(*[scal[t] for t in steps])
+    rates = [x * r for x, r in zip(lrs, rects)]
+    first = [1 if r == 0.0 else 0 for r in rects]
     with torch.cuda.device(dev):
         stream = N.stream_of(dev)
         if eight or masters is not None:
-            launch_adam(recs, pdt, eight, (b1, b2), weight_decay, eps, stream)
+            launch_adam([_ADAM.pack(*r) for r in zip(pp, gp, wp, mp, vp, msp, vsp, numels, seeds, rates, bc1, bc2, first)],
+                        pdt, eight, (b1, b2), weight_decay, eps, stream)
         else:
+            recs = [N.AdamTensor(*r) for r in zip(pp, gp, mp, vp, numels, rates, bc1, bc2, first)]
             N.check(N.load().thorn_adamw_multi(N.array(N.AdamTensor, recs), n, N.dtype_code(pdt), N.dtype_code(sdt),
                                                float(b1), float(b2), float(weight_decay), float(eps), stream),
                     "adamw_multi")
@@ -235,7 +259,8 @@ def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], sc
         m <- beta m + g  (rounded to 8 bits);   u = g + beta m;   x = u / (||u||_F + 1e-8)
 
     ``moments`` and ``scales`` as :func:`state8_zeros` with ``per_matrix=True`` makes them.
-    Returns the list of x (``out`` when given), which ``torch.ops.thorn_b200.polar_decomp`` takes.
+    Returns the list of x (``out`` when given, else views of one new allocation), which
+    ``torch.ops.thorn_b200.polar_decomp`` takes.
     """
     grads, moments, scales, out = _lists(grads=grads, moments=moments, scales=scales, out=out)
     n = len(grads)
@@ -248,19 +273,26 @@ def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], sc
     if not 0.0 <= beta < 1.0:
         raise ValueError(f"beta must be in [0, 1), got {beta}")
     seeds = _per_tensor(seeds, n, "seeds")
-    shapes = [g.shape for g in grads]
-    if any(len(s) < 2 for s in shapes):
+    shapes = list(map(_shape_of, grads))
+    if min(map(len, shapes)) < 2:
         raise ValueError("grads must be matrices or stacks of matrices")
     views = [(prod(s[:-2]), s[-2], s[-1]) for s in shapes]
-    _check(grads, pdt, dev, "grads", distinct=False)
-    _check(moments, CODES, dev, "moments", shapes)
-    _check(scales, SCALES, dev, "scales", [(B, _blocks(R * C)) for B, R, C in views])
-    if out is None:
-        out = [torch.empty(s, dtype=dtype, device=dev) for s in shapes]
+    gp = _check(grads, pdt, dev, "grads", distinct=False)
+    mp = _check(moments, CODES, dev, "moments", shapes)
+    sp = _check(scales, SCALES, dev, "scales", [(B, -(-R * C // BLOCK)) for B, R, C in views])
+    if out is None:  # views of one allocation, each starting on 16 bytes: 30 allocations cost more than the launch
+        starts, total = [], 0
+        for B, R, C in views:
+            starts.append(total)
+            total += (B * R * C + 7) // 8 * 8
+        flat = torch.empty(total, dtype=dtype, device=dev)
+        out = [flat.as_strided(s, _strides(s), a) for s, a in zip(shapes, starts)]
+        base = flat.data_ptr()
+        xp = [base + 2 * a for a in starts]
     else:
-        _check(out, dtype, dev, "out", shapes)
-    items = [(g.data_ptr(), m.data_ptr(), s.data_ptr(), x.data_ptr(), B, R, C, C, seed)
-             for g, m, s, x, (B, R, C), seed in zip(grads, moments, scales, out, views, seeds) if g.numel()]
+        xp = _check(out, dtype, dev, "out", shapes)
+    items = [(g, m, s, x, B, R, C, C, seed) for g, m, s, x, (B, R, C), seed in zip(gp, mp, sp, xp, views, seeds)
+             if B and R and C]
     if items:
         with torch.cuda.device(dev):
             launch_momentum8(items, pdt, dtype, float(beta), dev, N.stream_of(dev))
@@ -284,12 +316,11 @@ def apply_update_(params: Sequence[torch.Tensor], updates: Sequence[torch.Tensor
     if pdt not in _HALF or udt not in _HALF:
         raise TypeError(f"params and updates must be float16 or bfloat16, got {pdt} and {udt}")
     lrs = _per_tensor(lr, n, "lr")
-    shapes = [p.shape for p in params]
-    _check(params, pdt, dev, "params")
-    _check(updates, udt, dev, "updates", shapes, distinct=False)
-    _check(masters, torch.float32, dev, "masters", shapes)
-    items = [(u.data_ptr(), p.data_ptr(), w.data_ptr(), 0, 0, 1, 1, p.numel(), x)
-             for p, u, w, x in zip(params, updates, masters, lrs) if p.numel()]
+    shapes = list(map(_shape_of, params))
+    pp = _check(params, pdt, dev, "params")
+    up = _check(updates, udt, dev, "updates", shapes, distinct=False)
+    wp = _check(masters, torch.float32, dev, "masters", shapes)
+    items = [(u, p, w, 0, 0, 1, 1, k, x) for p, u, w, k, x in zip(pp, up, wp, map(_numel, params), lrs) if k]
     if items:
         with torch.cuda.device(dev):
             launch_apply(items, udt, pdt, weight_decay, N.stream_of(dev))
