@@ -291,3 +291,83 @@ def test_rounding_fractions_are_uniform():
             assert abs(np.corrcoef(f, base)[0, 1]) < 5 / np.sqrt(n)
     for lag in (4, 8, 128):
         assert abs(np.corrcoef(base[:-lag], base[lag:])[0, 1]) < 5 / np.sqrt(n)
+
+
+# ---------------------------------------------------------------------------------- THORN groups
+def _step(opt, *params, grad=None):
+    for p in params:
+        p.grad = torch.zeros_like(p) if grad is None else grad
+    opt.step()
+
+
+def test_group_options_are_checked_before_any_state():
+    from thorn_b200 import THORN
+
+    w = torch.nn.Parameter(torch.zeros(8, 8, dtype=torch.bfloat16))
+    f8 = torch.float8_e4m3fn
+    cases = [(dict(orthogonalize=False, master_weights=True, state_dtype=torch.bfloat16), ValueError),
+             (dict(orthogonalize=True, master_weights=True, state_dtype=torch.float16), ValueError),
+             (dict(orthogonalize=True, master_weights=True, decouple_md=True), NotImplementedError),
+             (dict(orthogonalize=False, master_weights=True, decouple_md=True), NotImplementedError)]
+    for opts, error in cases:
+        opt = THORN([{"params": [w], "lr": 1e-3, **opts}])
+        with pytest.raises(error):
+            _step(opt, w)
+        assert "step" not in opt.state[w]
+    sparse = torch.sparse_coo_tensor(torch.tensor([[1]]), torch.ones(1, 8, dtype=torch.bfloat16), (8, 8))
+    for opts in (dict(state_dtype=f8), dict(master_weights=True)):
+        opt = THORN([{"params": [w], "lr": 1e-3, "orthogonalize": False, **opts}])
+        with pytest.raises(NotImplementedError, match="sparse"):
+            _step(opt, w, grad=sparse)
+    t = torch.nn.Parameter(torch.zeros(8, 6, dtype=torch.bfloat16).T)
+    opt = THORN([{"params": [t], "lr": 1e-3, "orthogonalize": True, "state_dtype": f8}])
+    with pytest.raises(ValueError, match="contiguous"):
+        _step(opt, t)
+
+
+def test_state_layout_and_state_dict_round_trip():
+    """Keys, types and shapes of the state; a saved state comes back as it was (the base class
+    casts floating state to the parameter's dtype)."""
+    from thorn_b200 import THORN
+
+    f8, e8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+    def make():
+        torch.manual_seed(0)
+        ps = [torch.nn.Parameter(torch.randn(3, 10, 30).bfloat16()), torch.nn.Parameter(torch.randn(300).bfloat16())]
+        return ps, THORN([{"params": ps[:1], "lr": 1e-3, "orthogonalize": True, "state_dtype": f8, "master_weights": True},
+                          {"params": ps[1:], "lr": 1e-3, "orthogonalize": False, "state_dtype": f8}])
+
+    ps, opt = make()
+    for p in ps:
+        p.grad = torch.zeros_like(p)
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        opt.step()
+    a, b = opt.state[ps[0]], opt.state[ps[1]] if "step" in opt.state[ps[1]] else None
+    if b is None:
+        with pytest.raises(RuntimeError, match="CUDA devices only"):
+            opt.step(param=ps[1])
+        b = opt.state[ps[1]]
+    assert set(a) == {"step", "moment", "moment_scale", "rounding_seed", "master"}
+    assert set(b) == {"step", "moment", "moment_scale", "variance", "variance_scale", "rounding_seed"}
+    assert a["moment"].dtype is f8 and a["moment"].shape == (3, 10, 30) and a["moment_scale"].shape == (3, 3)
+    assert a["moment_scale"].dtype is e8 and a["master"].dtype is torch.float32
+    assert torch.equal(a["master"], ps[0].detach().float())
+    assert b["variance_scale"].shape == (3,) and (a["rounding_seed"], b["rounding_seed"]) == (0, 1 << 32)
+    gen = torch.Generator().manual_seed(1)
+    for st in (a, b):
+        for k in ("moment", "variance"):
+            if k in st:
+                st[k].view(torch.uint8).copy_(torch.randint(0, 127, st[k].shape, generator=gen, dtype=torch.uint8))
+                s = st[k + "_scale"]
+                s.view(torch.uint8).copy_(torch.randint(90, 120, s.shape, generator=gen, dtype=torch.uint8))
+    a["master"] += 1e-6
+    ps2, opt2 = make()
+    opt2.load_state_dict(opt.state_dict())
+    for p, q in zip(ps, ps2):
+        for k, v in opt.state[p].items():
+            w = opt2.state[q][k]
+            if isinstance(v, torch.Tensor):
+                assert w.dtype is v.dtype and torch.equal(w.view(torch.uint8), v.view(torch.uint8)), k
+            else:
+                assert w == v

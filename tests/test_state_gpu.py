@@ -430,3 +430,249 @@ def test_capture_is_refused():
             T.momentum_(g, m, s, beta=0.9, seeds=[1])
     graph.replay()
     torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------------- THORN groups
+F8 = torch.float8_e4m3fn
+
+
+def _params(shapes, dtype, seed):
+    torch.manual_seed(seed)
+    return [torch.nn.Parameter((torch.randn(s, device="cuda") * 0.02).to(dtype)) for s in shapes]
+
+
+def _grads(params, seed):
+    torch.manual_seed(seed)
+    return [(torch.randn(p.shape, device="cuda") * 1e-3).to(p.dtype) for p in params]
+
+
+@pytest.mark.parametrize("opts", [dict(state_dtype=F8), dict(state_dtype=F8, master_weights=True),
+                                  dict(master_weights=True), dict(state_dtype=F8, rectify=True, eps=1e-8)])
+def test_adam_group_steps_like_the_function(opts):
+    """Four steps of a (R)AdamW group are four calls of adamw_, bit for bit."""
+    import thorn_b200 as T
+
+    shapes = [(1000,), (33, 130), (5,)]
+    p = _params(shapes, torch.bfloat16, 1)
+    q = [t.detach().clone() for t in p]
+    opt = T.THORN([{"orthogonalize": False, "params": p, "lr": 1e-2, **opts}])
+    kw = {k: opts[k] for k in ("rectify", "eps") if k in opts}
+    if "master_weights" in opts:
+        kw["masters"] = [t.float() for t in q]
+    if "state_dtype" in opts:
+        st = [T.state8_zeros(t) for t in q + q]
+        m, v = [c for c, _ in st[:3]], [c for c, _ in st[3:]]
+        kw.update(moment_scales=[s for _, s in st[:3]], variance_scales=[s for _, s in st[3:]])
+    else:
+        m, v = [torch.zeros(s, device="cuda") for s in shapes], [torch.zeros(s, device="cuda") for s in shapes]
+    for step in range(1, 5):
+        g = _grads(p, 10 + step)
+        for t, x in zip(p, g):
+            t.grad = x.clone()
+        opt.step()
+        seeds = [(i << 32) + step for i in range(3)] if "state_dtype" in opts else None
+        T.adamw_(q, g, m, v, step=step, lr=1e-2, seeds=seeds, **kw)
+        for i, t in enumerate(p):
+            assert torch.equal(t.detach(), q[i]), (step, i)
+            assert np.array_equal(u8(opt.state[t]["moment"]), u8(m[i]))
+            assert np.array_equal(u8(opt.state[t]["variance"]), u8(v[i]))
+            if "masters" in kw:
+                assert torch.equal(opt.state[t]["master"], kw["masters"][i])
+
+
+def _newton_schulz(x, conf):
+    """The library's Newton-Schulz result for the inputs x (matrices or stacks), in x's dtype."""
+    import ctypes
+
+    from thorn_b200 import _native as N
+
+    lib = N.load()
+    R_, C_ = x.shape[-2:]
+    B = x.numel() // (R_ * C_)
+    ld = int(lib.thorn_ns_ld(C_))
+    X = torch.zeros((B, R_, ld), dtype=x.dtype, device="cuda")
+    X[:, :, :C_] = x.reshape(B, R_, C_)
+    out = torch.empty((B, R_, C_), dtype=x.dtype, device="cuda")
+    wsb = int(lib.thorn_ns_workspace_bytes(B, R_, C_))
+    ws = torch.empty(max(256, wsb), dtype=torch.uint8, device="cuda")
+    co = (ctypes.c_double * (3 * conf.iters))(*[v for abc in conf.coeffs[:conf.iters] for v in abc])
+    rs = (ctypes.c_int32 * max(1, len(conf.restarts)))(*conf.restarts)
+    N.check(lib.thorn_ns_batched(X.data_ptr(), out.data_ptr(), ws.data_ptr(), wsb, B, R_, C_, N.dtype_code(x.dtype), co,
+                                 conf.iters, rs, len(conf.restarts), None, N.stream_of(X.device)), "ns_batched")
+    return out.reshape(x.shape)
+
+
+@pytest.mark.parametrize("ns_dtype", [torch.float16, torch.bfloat16])
+def test_ortho_group_with_8_bit_momentum_and_masters(ns_dtype):
+    """Two steps: the momentum is momentum_'s bit for bit, and the masters move by the library's
+    Newton-Schulz result for momentum_'s input, up to the fp32 roundings of the apply (one
+    matrix has rows that need padding, one stack has 3 dimensions); the parameter is the
+    rounded master."""
+    import thorn_b200 as T
+    from thorn_b200.optimizer import GroupConfig
+
+    shapes = [(64, 96), (40, 37), (3, 16, 24), (128, 256)]
+    p = _params(shapes, torch.bfloat16, 2)
+    opt = T.THORN([{"orthogonalize": True, "params": p, "lr": 1e-2, "weight_decay": 0.0, "betas": (0.9, 0.0),
+                    "state_dtype": F8, "master_weights": True}])
+    opt.ns_dtype = ns_dtype
+    conf = GroupConfig.from_kwargs(**opt.param_groups[0])
+    st = [T.state8_zeros(t, per_matrix=True) for t in p]
+    for step in range(1, 3):
+        g = _grads(p, 20 + step)
+        before = [opt.state[t]["master"].clone() if step > 1 else t.detach().float() for t in p]
+        for t, x in zip(p, g):
+            t.grad = x.clone()
+        opt.step()
+        x = T.momentum_(g, [c for c, _ in st], [s for _, s in st], beta=0.9, dtype=ns_dtype,
+                        seeds=[(i << 32) + step for i in range(4)])
+        for i, t in enumerate(p):
+            s = opt.state[t]
+            assert np.array_equal(u8(s["moment"]), u8(st[i][0])) and np.array_equal(u8(s["moment_scale"]), u8(st[i][1]))
+            lr = 1e-2 * conf.lr_scale(*t.shape[-2:])
+            want = before[i].double() - lr * _newton_schulz(x[i], conf).double()
+            # the rate rounded to fp32, one fma
+            assert bool(((s["master"] - want).abs() <= 2 * E * (before[i].abs() + (want - before[i]).abs())).all()), (step, i)
+            assert torch.equal(t.detach(), s["master"].bfloat16())
+    assert not opt.device_error()
+
+
+def test_masters_follow_fp32_parameters():
+    """bf16 parameters with masters against fp32 parameters of the same values and gradients:
+    both groups' masters are the fp32 run's parameters up to fp32 rounding (tall matrices with
+    their per-neuron norm among them)."""
+    import thorn_b200 as T
+
+    ortho, adam = [(96, 64), (64, 64), (257, 40)], [(500,), (10, 30)]
+    a = _params(ortho + adam, torch.bfloat16, 3)
+    b = [torch.nn.Parameter(t.detach().float()) for t in a]
+
+    def make(ps, **kw):
+        return T.THORN([{"orthogonalize": True, "params": ps[:3], "lr": 1e-2, **kw},
+                        {"orthogonalize": False, "params": ps[3:], "lr": 1e-2, **kw}])
+
+    oa, ob = make(a, master_weights=True), make(b)
+    start = [t.detach().clone() for t in b]
+    for step in range(3):
+        for t, u, x in zip(a, b, _grads(a, 30 + step)):
+            t.grad, u.grad = x.clone(), x.float()
+        oa.step()
+        ob.step()
+    for i, (t, u) in enumerate(zip(a, b)):
+        m = oa.state[t]["master"]
+        assert oa.state[t]["moment"].dtype is torch.float32
+        moved = (u.detach() - start[i]).abs()
+        # AdamW: the update's arithmetic differs by at most 16 roundings per step; the apply of the
+        # orthogonalised group is the same arithmetic
+        assert bool(((m - u.detach()).abs() <= 3 * 16 * E * (u.detach().abs() + moved + 1e-2)).all()), i
+        assert torch.equal(t.detach(), m.bfloat16())
+
+
+def test_8_bit_state_survives_saving():
+    """Four steps against two, a save, a load into a new optimizer and two: the same bits."""
+    import thorn_b200 as T
+
+    shapes = [(48, 64), (200,)]
+
+    def make():
+        p = _params(shapes, torch.bfloat16, 4)
+        return p, T.THORN([{"orthogonalize": True, "params": p[:1], "lr": 1e-2, "state_dtype": F8, "master_weights": True},
+                           {"orthogonalize": False, "params": p[1:], "lr": 1e-2, "state_dtype": F8}])
+
+    def run(p, opt, steps):
+        for k in steps:
+            for t, x in zip(p, _grads(p, 40 + k)):
+                t.grad = x
+            opt.step()
+
+    p, opt = make()
+    run(p, opt, range(4))
+    q, opt2 = make()
+    run(q, opt2, range(2))
+    saved = opt2.state_dict()
+    r, opt3 = make()
+    for t, u in zip(r, q):
+        t.data.copy_(u.data)
+    opt3.load_state_dict(saved)
+    run(r, opt3, range(2, 4))
+    for t, u in zip(p, r):
+        assert torch.equal(t.detach(), u.detach())
+        for k, v in opt.state[t].items():
+            if isinstance(v, torch.Tensor):
+                assert np.array_equal(u8(v), u8(opt3.state[u][k])), k
+
+
+@pytest.mark.parametrize("ortho", [True, False])
+def test_update_rate_advances_the_state_only(ortho):
+    import thorn_b200 as T
+
+    p = _params([(64, 200)], torch.bfloat16, 5)
+    opt = T.THORN([{"orthogonalize": ortho, "params": p, "lr": 1e-2, "state_dtype": F8, "master_weights": True}])
+    opt._update_rate = 2
+    moved, codes = [], []
+    for k in range(4):
+        before = p[0].detach().clone()
+        p[0].grad = _grads(p, 50 + k)[0]
+        opt.step()
+        moved.append(not torch.equal(before, p[0].detach()))
+        codes.append(u8(opt.state[p[0]]["moment"]).copy())
+    assert moved == [True, False, True, False]  # applied where (step + 1) is a multiple of the rate
+    assert all(not np.array_equal(a, b) for a, b in zip(codes, codes[1:]))
+
+
+@pytest.mark.parametrize("ortho", [True, False])
+def test_decoupled_magnitudes_and_magma_with_8_bit_state(ortho):
+    """decouple_md and momentum_align with 8-bit state.  From zero state and unit gains the
+    first momentum is (1 - beta1 for AdamW, 1 for the orthogonalised group) times the gradient to
+    within a code's step (2^-3 of the value), and the steps stay finite and move the parameters."""
+    import thorn_b200 as T
+
+    torch.manual_seed(9)
+    p = _params([(64, 48), (40, 56)], torch.float32, 6)
+    g = _grads(p, 60)
+    opt = T.THORN([{"orthogonalize": ortho, "params": p, "lr": 1e-2, "decouple_md": True, "momentum_align": True,
+                    "state_dtype": F8, "betas": (0.9, 0.95)}])
+    before = [t.detach().clone() for t in p]
+    for k in range(3):
+        for t, x in zip(p, g):
+            t.grad = x.clone()
+        opt.step()
+        if k == 0:
+            for t, x in zip(p, g):
+                m = T.state8_read(opt.state[t]["moment"], opt.state[t]["moment_scale"])
+                want = x if ortho else 0.1 * x
+                size = opt.state[t]["moment_scale"].float().max()
+                # a gain of softplus(0.5413) = 1 to a rounding
+                assert bool(((m - want).abs() <= want.abs() * (2.0 ** -3 + 2.0 ** -10) + size * 2.0 ** -9).all())
+    assert all(bool(t.isfinite().all()) for t in p)
+    assert any(not torch.equal(t.detach(), b) for t, b in zip(p, before))
+
+
+def test_functions_chained_as_one_step():
+    """momentum_ -> polar_decomp -> apply_update_ beside adamw_: two steps of a small model by the
+    functions alone land where THORN's groups do (2e-2 of the movement in the Frobenius norm for
+    the matrix, as the other Newton-Schulz tests: the operator normalises its input once more)."""
+    import thorn_b200 as T
+    from thorn_b200.optimizer import GroupConfig
+
+    p = _params([(64, 96), (96,)], torch.bfloat16, 8)
+    w0 = p[0].detach().float()
+    opts = dict(lr=1e-2, state_dtype=F8, master_weights=True)
+    opt = T.THORN([{"orthogonalize": True, "params": p[:1], **opts}, {"orthogonalize": False, "params": p[1:], **opts}])
+    conf = GroupConfig.from_kwargs(**opt.param_groups[0])
+    flat = [float(x) for abc in conf.coeffs[:conf.iters] for x in abc]
+    a, b = [t.detach().clone() for t in p]
+    wa, wb = a.float(), b.float()
+    (mc, ms), (nc, ns), (vc, vs) = T.state8_zeros(a, per_matrix=True), T.state8_zeros(b), T.state8_zeros(b)
+    for step in range(1, 3):
+        ga, gb = _grads(p, 80 + step)
+        p[0].grad, p[1].grad = ga.clone(), gb.clone()
+        opt.step()
+        x, = T.momentum_([ga], [mc], [ms], beta=0.9, seeds=[step])
+        u = torch.ops.thorn_b200.polar_decomp(x, flat, list(conf.restarts))
+        T.apply_update_([a], [u], masters=[wa], lr=1e-2 * conf.lr_scale(64, 96), weight_decay=0.1)
+        T.adamw_([b], [gb], [nc], [vc], step=step, lr=1e-2, moment_scales=[ns], variance_scales=[vs], masters=[wb],
+                 seeds=[(1 << 32) + step])
+    assert torch.equal(b, p[1].detach()) and torch.equal(wb, opt.state[p[1]]["master"])
+    moved = opt.state[p[0]]["master"] - w0
+    assert C.rel_fro((wa - w0).cpu().numpy(), moved.cpu().numpy()) <= 2e-2

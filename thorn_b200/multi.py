@@ -101,12 +101,16 @@ _device_index, _contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
 _pointer, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
 
 
-def _device(t) -> torch.device:
-    if t.device.type != "cuda":
-        raise RuntimeError(f"thorn_b200 runs its step on CUDA devices only; got a tensor on {t.device}")
+def refuse_capture() -> None:
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("this call takes host scalars (step, learning rate, seeds) that a captured CUDA graph would "
                            "repeat at every replay: call it outside of graph capture")
+
+
+def _device(t) -> torch.device:
+    if t.device.type != "cuda":
+        raise RuntimeError(f"thorn_b200 runs its step on CUDA devices only; got a tensor on {t.device}")
+    refuse_capture()
     return t.device
 
 

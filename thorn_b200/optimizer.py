@@ -19,7 +19,13 @@ no CPU path.
 
 Extensions (all optional, off by default):
 * group key ``state_dtype``: dtype of the optimizer state (the reference keeps
-  it in the parameter dtype);
+  it in the parameter dtype); ``torch.float8_e4m3fn`` keeps it in 8 bits (codes
+  under the reference's keys, one power of two per 128 elements under
+  ``moment_scale`` / ``variance_scale``, stochastic rounding from
+  ``rounding_seed`` and the step; see :mod:`thorn_b200.multi`);
+* group key ``master_weights``: 16-bit parameters get an fp32 copy, state key
+  ``master``, that takes the updates; the parameter receives its rounding.  The
+  moments are then fp32, or 8 bits with the key above;
 * attribute ``ns_dtype``: operand type of the Newton-Schulz GEMMs,
   ``torch.float16`` (the reference's choice, thorn.py:634-635) or
   ``torch.bfloat16``.
@@ -39,6 +45,7 @@ from torch.distributed.tensor import DTensor, Replicate
 from torch.optim import Optimizer
 
 from . import _native as N
+from . import multi
 from .coeffs import gram_ns_restarts, optimal_composition
 
 __all__ = ["THORN", "THORNOrthoGroup", "THORNNonOrthoGroup", "THORNGroup"]
@@ -285,7 +292,7 @@ class _Arena:
 class _Item:
     __slots__ = ("p", "g", "state", "B", "R", "C", "apply", "pdt", "sdt", "normsq", "rs", "cs", "sig_r", "sig_c",
                  "rgs", "cgs", "rs_new", "cs_new", "pnorm", "scalar", "ggrad_r", "ggrad_c", "split", "scale",
-                 "m_rows", "v_rows", "row_norm")
+                 "m_rows", "v_rows", "row_norm", "master")
 
 
 class THORN(Optimizer):
@@ -412,11 +419,23 @@ class THORN(Optimizer):
 
     # ------------------------------------------------------------- routing
     def _init_state(self, p, state, cfg: GroupConfig, gdict):
+        master = bool(gdict.get("master_weights")) and p.dtype in (torch.bfloat16, torch.float16)
+        sdt = gdict.get("state_dtype") or (torch.float32 if master else p.dtype)
+        eight = sdt is multi.CODES
+        self._check_state_options(p, cfg, sdt, master)
         state["step"] = 1
-        sdt = gdict.get("state_dtype") or p.dtype
-        state["moment"] = torch.zeros_like(p, dtype=sdt)
-        if not cfg.orthogonalize:
-            state["variance"] = torch.zeros_like(p, dtype=sdt)
+        if eight:
+            state["moment"], state["moment_scale"] = multi.state8_zeros(p, per_matrix=cfg.orthogonalize)
+            if not cfg.orthogonalize:
+                state["variance"], state["variance_scale"] = multi.state8_zeros(p)
+            # the place of the parameter in the optimizer, so that replicas round alike
+            state["rounding_seed"] = self._place_of(p) << 32
+        else:
+            state["moment"] = torch.zeros_like(p, dtype=sdt)
+            if not cfg.orthogonalize:
+                state["variance"] = torch.zeros_like(p, dtype=sdt)
+        if master:
+            state["master"] = p.detach().float()
         if cfg.decouple_md:
             if p.ndim > 1 and cfg.split_gain:
                 if isinstance(p, DTensor) and not all(isinstance(pl, Replicate) for pl in p.placements):
@@ -453,6 +472,51 @@ class THORN(Optimizer):
             state["random_state"] = seed
             state["s"] = torch.ones((), dtype=p.dtype, device=_local(p).device)
 
+    @staticmethod
+    def _check_state_options(p, cfg: GroupConfig, sdt, master: bool) -> None:
+        """Refuses what 8-bit state and master weights are not implemented for."""
+        eight = sdt is multi.CODES
+        if not (eight or master):
+            return
+        if master and not eight and sdt is not torch.float32:
+            raise ValueError(f"master_weights needs fp32 or 8-bit state, got state_dtype={sdt}")
+        if master and cfg.decouple_md:
+            raise NotImplementedError("master_weights with decouple_md is not implemented by thorn_b200")
+        if eight and isinstance(p, DTensor):
+            raise NotImplementedError("8-bit state of DTensor parameters is not implemented by thorn_b200")
+        if isinstance(p, DTensor) and cfg.orthogonalize and not all(isinstance(q, Replicate) for q in p.placements):
+            raise NotImplementedError("master_weights of sharded orthogonalized parameters is not implemented by "
+                                      "thorn_b200")
+        if not p.is_contiguous():
+            raise ValueError("thorn_b200 needs contiguous parameters")
+
+    def _place_of(self, p) -> int:
+        i = 0
+        for group in self.param_groups:
+            for q in group["params"]:
+                if q is p:
+                    return i
+                i += 1
+        return i
+
+    @staticmethod
+    def _rounding_seed(st) -> int:
+        """Seed of a parameter's 8-bit rounding at this step."""
+        return (int(st["rounding_seed"]) + int(st["step"])) & _U64
+
+    def load_state_dict(self, state_dict) -> None:
+        """``Optimizer.load_state_dict``, which casts state to the parameter's dtype, with the
+        8-bit codes and scales and the fp32 state beside master weights as they were saved."""
+        super().load_state_dict(state_dict)
+        saved = [k for g in state_dict["param_groups"] for k in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for k, p in zip(saved, params):
+            old = state_dict["state"].get(k, {})
+            if "moment_scale" in old or "master" in old:
+                for key in ("moment", "variance", "moment_scale", "variance_scale", "master"):
+                    if key in old:
+                        self.state[p][key] = old[key].to(device=p.device)
+
     def _magma(self, items, cfg, recovered: bool, group=None) -> None:
         """Magma masking (thorn.py:806-836) for a list of launch records.
 
@@ -472,6 +536,9 @@ class THORN(Optimizer):
             it.scale = 1.0
         if not cfg.momentum_align or not items:
             return
+        for it in items:
+            if "moment_scale" in it.state:
+                it.m_rows = multi.state8_read(it.state["moment"], it.state["moment_scale"])
         stats = self._magma_stats(items, cfg, recovered)
         scores = self._magma_scores(items, stats, group)
         for it, v in zip(items, scores):
@@ -572,11 +639,16 @@ class THORN(Optimizer):
                 if cfg.orthogonalize or isinstance(p.data, DTensor):
                     raise NotImplementedError("sparse gradients are implemented for (R)AdamW parameters on one "
                                               "device only")
+                if gdict.get("state_dtype") is multi.CODES or gdict.get("master_weights"):
+                    raise NotImplementedError("sparse gradients with 8-bit state or master weights are not implemented "
+                                              "by thorn_b200")
                 if cfg.decouple_md or p.grad.sparse_dim() != 1:
                     p.grad = p.grad.to_dense()  # thorn.py:1667-1668
             state = self.state[p]
             if "step" not in state:
                 self._init_state(p, state, cfg, gdict)
+            if ("moment_scale" in state or "master" in state) and _local(p).device.type == "cuda":
+                multi.refuse_capture()
             is_sharded = isinstance(p.data, DTensor) and not all(isinstance(pl, Replicate) for pl in p.placements)
             if is_sharded and cfg.orthogonalize:
                 sharded.append(p)
@@ -673,7 +745,10 @@ class THORN(Optimizer):
             it.apply = (st["step"] + 1) % self._update_rate == 0
             it.pdt = it.p.dtype
             it.sdt = _local(st["moment"]).dtype
-            N.dtype_code(it.pdt), N.dtype_code(it.sdt)
+            it.master = _local(st["master"]) if "master" in st else None
+            N.dtype_code(it.pdt)
+            if "moment_scale" not in st:
+                N.dtype_code(it.sdt)
             if g.dtype != it.pdt:
                 raise TypeError(f"gradient dtype {g.dtype} differs from parameter dtype {it.pdt}")
             it.normsq = arena.alloc(it.B, red1) if ortho else None
@@ -832,9 +907,9 @@ class THORN(Optimizer):
         buckets: dict = {}
         for it in items:
             if it.apply:
-                buckets.setdefault((it.R, it.C, it.pdt, it.sdt), []).append(it)
+                buckets.setdefault((it.R, it.C, it.pdt, it.sdt, it.master is not None), []).append(it)
         chunks = []
-        for (R, C, pdt, sdt), its in buckets.items():
+        for (R, C, pdt, sdt, _), its in buckets.items():
             cap = max(1, self.polar_decomp_batch_size // max(1, R * C)) if self.polar_decomp_batch_size > 0 else 1
             cap = balanced_cap(sum(it.B for it in its), cap)
             cur, n = [], 0
@@ -857,8 +932,12 @@ class THORN(Optimizer):
             self._md_prep(items, arena, new=False, stream=stream)
         write_grad = 1 if (md and not cfg.none_grad) else 0
         by_dt: dict = {}
-        scr = self._scratch(dev, [lib.thorn_ortho_pre_scratch_bytes(it.B, it.R, it.C, 1 if md else 0) for it in items])
-        for it, sp in zip(items, scr):
+        eights = [it for it in items if it.sdt is multi.CODES]
+        wide = [it for it in items if it.sdt is not multi.CODES]
+        if eights and md:
+            self._recover_eights(eights, arena, stream)
+        scr = self._scratch(dev, [lib.thorn_ortho_pre_scratch_bytes(it.B, it.R, it.C, 1 if md else 0) for it in wide])
+        for it, sp in zip(wide, scr):
             t = N.OrthoPreTensor(it.p.data_ptr() if md else None, it.g.data_ptr(), _local(it.state["moment"]).data_ptr(),
                                  arena.ptr(it.normsq), it.B, it.R, it.C,
                                  arena.ptr(it.rs) if md else None, arena.ptr(it.cs) if md else None,
@@ -871,9 +950,11 @@ class THORN(Optimizer):
             N.check(lib.thorn_ortho_pre_multi(N.array(N.OrthoPreTensor, ts), len(ts), N.dtype_code(pdt),
                                               N.dtype_code(sdt), N.dtype_code(udt), b1, 1 if md else 0, write_grad,
                                               stream), "ortho_pre_multi")
-        self._profile_end(self.profile_momentum, ev, self._momentum_bytes(items, md))
+        self._profile_end(self.profile_momentum, ev, self._momentum_bytes(wide, md))
         if md:
             self._md_gains(items, cfg, arena, stream)
+        # 8-bit momentum that no Newton-Schulz input follows in this step
+        self._momentum_eights([it for it in eights if not it.apply], None, b1, dev, stream)
 
         coeffs = (ctypes.c_double * (3 * max(1, cfg.iters)))(*[x for abc in cfg.coeffs[:cfg.iters] for x in abc])
         rs = list(cfg.restarts)
@@ -885,15 +966,19 @@ class THORN(Optimizer):
             U = torch.empty((nb, R, C), dtype=self.ns_dtype, device=dev)
             casts, off = [], 0
             esz = X.element_size()
-            for it in its:
+            if sdt is multi.CODES:
+                self._momentum_eights(its, X, b1, dev, stream)
+            for it in its if sdt is not multi.CODES else ():
                 casts.append(N.NsCastTensor(it.g.data_ptr(), _local(it.state["moment"]).data_ptr(), arena.ptr(it.normsq),
                                             X.data_ptr() + off * R * ldc * esz, it.B, it.R, it.C,
                                             arena.ptr(it.rs) if md else None, arena.ptr(it.cs) if md else None,
                                             1 if (md and not it.split) else 0, 1 if (md and not write_grad) else 0))
                 off += it.B
             udt = pdt if pdt == sdt else torch.float32
-            N.check(lib.thorn_ns_cast_multi(N.array(N.NsCastTensor, casts), len(casts), N.dtype_code(pdt),
-                                            N.dtype_code(sdt), N.dtype_code(udt), ns_code, b1, stream), "ns_cast_multi")
+            if casts:
+                N.check(lib.thorn_ns_cast_multi(N.array(N.NsCastTensor, casts), len(casts), N.dtype_code(pdt),
+                                                N.dtype_code(sdt), N.dtype_code(udt), ns_code, b1, stream),
+                        "ns_cast_multi")
             wsb = int(lib.thorn_ns_workspace_bytes(nb, R, C))
             ws = torch.empty(max(256, wsb), dtype=torch.uint8, device=dev)
             if self.profile_ns is not None:
@@ -914,11 +999,24 @@ class THORN(Optimizer):
                 row_scale, mat_stats = arena.get(rsh), arena.get(msh)
                 (sp,) = self._scratch(dev, [lib.thorn_pnn_scratch_bytes(nb, R)])
                 pt = N.PnnTensor(U.data_ptr(), row_scale.data_ptr(), mat_stats.data_ptr(), nb, R, C, sp, 0)
-                N.check(lib.thorn_pnn_stats_multi(N.array(N.PnnTensor, [pt]), 1, ns_code, N.dtype_code(pdt), stream),
+                # with master weights the parameters' type is fp32
+                pnn_code = N.F32 if its[0].master is not None else N.dtype_code(pdt)
+                N.check(lib.thorn_pnn_stats_multi(N.array(N.PnnTensor, [pt]), 1, ns_code, pnn_code, stream),
                         "pnn_stats_multi")
             posts, off = [], 0
             usz = U.element_size()
             lr_eff = float(cfg.lr) * cfg.lr_scale(R, C)
+            if its[0].master is not None:
+                applies = []
+                for it in its:
+                    applies.append((U.data_ptr() + off * R * C * usz, it.p.data_ptr(), it.master.data_ptr(),
+                                    0 if row_scale is None else row_scale.data_ptr() + off * R * 4,
+                                    0 if mat_stats is None else mat_stats.data_ptr() + off * 2 * 4, it.B, R, C,
+                                    lr_eff * it.scale))
+                    off += it.B
+                multi.launch_apply(applies, self.ns_dtype, pdt, cfg.weight_decay, stream)
+                del U
+                continue
             scr = self._scratch(dev, [lib.thorn_sumsq_scratch_bytes(it.B, R, C) if md else 0 for it in its])
             for it, sp in zip(its, scr):
                 posts.append(N.OrthoPostTensor(
@@ -936,6 +1034,39 @@ class THORN(Optimizer):
             keep = self._md_finalize(items, arena, lambda it: True, stream)
         self._finish(params, cfg)
         del keep
+
+    def _recover_eights(self, items, arena, stream):
+        """Direction recovery (thorn.py:890-908) of tensors whose momentum is held in 8 bits: the
+        recovered gradient is stored, and the momentum pass reads it."""
+        lib = N.load()
+        scr = self._scratch(items[0].p.device,
+                            [lib.thorn_ortho_pre_scratch_bytes(it.B, it.R, it.C, 1) for it in items])
+        by_dt: dict = {}
+        for it, sp in zip(items, scr):
+            by_dt.setdefault(it.pdt, []).append(N.OrthoPreTensor(
+                it.p.data_ptr(), it.g.data_ptr(), None, None, it.B, it.R, it.C, arena.ptr(it.rs), arena.ptr(it.cs),
+                0 if it.split else 1, arena.ptr(it.rgs), arena.ptr(it.cgs), sp))
+        for pdt, ts in by_dt.items():
+            code = N.dtype_code(pdt)
+            N.check(lib.thorn_ortho_pre_multi(N.array(N.OrthoPreTensor, ts), len(ts), code, code, code, 0.0, 1, 1,
+                                              stream), "md recover_direction")
+
+    def _momentum_eights(self, items, X, b1: float, dev, stream):
+        """8-bit momentum of ``items`` (one parameter dtype when X is given) and their inputs in X."""
+        by_dt: dict = {}
+        off = 0
+        for it in items:
+            st = it.state
+            ptr = ldx = 0
+            if X is not None:
+                ldx = X.shape[-1]
+                ptr = X.data_ptr() + off * it.R * ldx * X.element_size()
+                off += it.B
+            by_dt.setdefault(it.pdt, []).append((it.g.data_ptr(), st["moment"].data_ptr(),
+                                                 st["moment_scale"].data_ptr(), ptr, it.B, it.R, it.C, ldx or it.C,
+                                                 self._rounding_seed(st)))
+        for pdt, ts in by_dt.items():
+            multi.launch_momentum8(ts, pdt, self.ns_dtype, b1, dev, stream)
 
     # ------------------------------------------------------- (R)AdamW group
     def _sparse_rows(self, params, cfg):
@@ -1026,17 +1157,31 @@ class THORN(Optimizer):
                 t = N.OrthoPreTensor(it.p.data_ptr(), it.g.data_ptr(), None, None, it.B, it.R, it.C,
                                      arena.ptr(it.rs), arena.ptr(it.cs), 0 if it.split else 1,
                                      arena.ptr(it.rgs), arena.ptr(it.cgs), sp)
-                by_dt.setdefault((it.pdt, it.sdt), []).append(t)
+                # without a moment the state's type is not used
+                by_dt.setdefault((it.pdt, it.pdt if it.sdt is multi.CODES else it.sdt), []).append(t)
             for (pdt, sdt), ts in by_dt.items():
                 N.check(lib.thorn_ortho_pre_multi(N.array(N.OrthoPreTensor, ts), len(ts), N.dtype_code(pdt),
                                                   N.dtype_code(sdt), N.dtype_code(pdt), float(b1), 1, 1, stream),
                         "md recover_direction")
-        by_dt = {}
+        by_dt, by_state = {}, {}
         for it in items:
             step = it.state["step"]
             rect = cfg.rect(step)
             bc1 = 1 / (1 - b1 ** step)
             bc2 = 1 / (1 - b2 ** step)
+            st = it.state
+            if "moment_scale" in st or it.master is not None:
+                eight = "moment_scale" in st
+                if not eight and it.sdt is not torch.float32:
+                    raise TypeError(f"master weights need fp32 or 8-bit moments, got {it.sdt}")
+                by_state.setdefault((it.pdt, eight), []).append(multi.adam_record(
+                    it.p.data_ptr() if it.apply else 0, it.g.data_ptr(),
+                    0 if it.master is None else it.master.data_ptr(), _local(st["moment"]).data_ptr(),
+                    _local(st["variance"]).data_ptr(), st["moment_scale"].data_ptr() if eight else 0,
+                    st["variance_scale"].data_ptr() if eight else 0, it.p.numel(),
+                    self._rounding_seed(st) if eight else 0, float(cfg.lr) * rect * it.scale, bc1, bc2,
+                    1 if rect == 0.0 else 0))
+                continue
             t = N.AdamTensor(it.p.data_ptr() if it.apply else None, it.g.data_ptr(),
                              _local(it.state["moment"]).data_ptr(), _local(it.state["variance"]).data_ptr(),
                              it.p.numel(), float(cfg.lr) * rect * it.scale, bc1, bc2, 1 if rect == 0.0 else 0)
@@ -1045,6 +1190,8 @@ class THORN(Optimizer):
             N.check(lib.thorn_adamw_multi(N.array(N.AdamTensor, ts), len(ts), N.dtype_code(pdt), N.dtype_code(sdt),
                                           float(b1), float(b2), float(cfg.weight_decay), float(cfg.eps), stream),
                     "adamw_multi")
+        for (pdt, eight), recs in by_state.items():
+            multi.launch_adam(recs, pdt, eight, (b1, b2), cfg.weight_decay, cfg.eps, stream)
         keep = None
         if md:
             self._md_gains(items, cfg, arena, stream)
