@@ -6,6 +6,7 @@ call raises.  There is no CPU or eager-PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p
@@ -180,6 +181,25 @@ def load(build_if_missing: bool = False):
             fn.argtypes = args
         _lib = lib
         return lib
+
+
+_host = None
+
+
+def host():
+    """The host extension (csrc/host_records.cpp); raises if it is not built."""
+    global _host
+    if _host is None:
+        with _lock:
+            if _host is None:
+                if not os.path.exists(_build.HOST_LIB):
+                    raise RuntimeError(f"thorn_b200 host extension not found at {_build.HOST_LIB}; build it with "
+                                       "`python -m thorn_b200.build`")
+                spec = importlib.util.spec_from_file_location("thorn_b200_host", _build.HOST_LIB)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _host = module
+    return _host
 
 
 def check(status: int, what: str):

@@ -1,8 +1,8 @@
-"""Build the sm_100a shared library ``thorn_b200/_lib/libthorn_b200.so`` with nvcc.
+"""Build the sm_100a shared library ``thorn_b200/_lib/libthorn_b200.so`` with nvcc, and the
+host extension ``thorn_b200/_lib/thorn_b200_host.so`` (``csrc/host_records.cpp``) with g++.
 
-Usage: ``python -m thorn_b200.build [--force]``.  The library is built in-tree
-so it travels with the checkout; it is rebuilt when a source or header is
-newer than the library.
+Usage: ``python -m thorn_b200.build [--force]``.  Both are built in-tree so they
+travel with the checkout; each is rebuilt when a source or header is newer.
 """
 from __future__ import annotations
 
@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -18,6 +19,8 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIB_DIR, "libthorn_b200.so")
+HOST_LIB = os.path.join(LIB_DIR, "thorn_b200_host.so")
+HOST_SRC = os.path.join(CSRC, "host_records.cpp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -46,7 +49,29 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def build_host(force: bool = False, verbose: bool = False) -> str:
+    """The CPython extension over this interpreter's libtorch."""
+    if not force and os.path.exists(HOST_LIB) and os.path.getmtime(HOST_LIB) >= os.path.getmtime(HOST_SRC):
+        return HOST_LIB
+    import torch
+
+    os.makedirs(LIB_DIR, exist_ok=True)
+    root = os.path.dirname(torch.__file__)
+    tmp = HOST_LIB + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I", sysconfig.get_paths()["include"], HOST_SRC, "-L", os.path.join(root, "lib"), "-ltorch_python",
+           "-ltorch_cpu", "-lc10", "-o", tmp]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, HOST_LIB)
+    return HOST_LIB
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    build_host(force, verbose)
     if not force and not _stale():
         return LIB
     os.makedirs(LIB_DIR, exist_ok=True)

@@ -25,10 +25,9 @@ the parameter's dtype (thorn.py:1591-1599) and updates 16-bit parameters in plac
 from __future__ import annotations
 
 import struct
+from contextlib import nullcontext
 from functools import lru_cache
-from itertools import repeat
 from math import prod
-from operator import attrgetter
 from typing import Optional, Sequence, Union
 
 import torch
@@ -50,7 +49,14 @@ _APPLY = struct.Struct("<5Q3qf4x")
 
 
 def _records(struct_type, parts):
+    """A C array of records: from a list of packed ones, or over a buffer that holds them."""
+    if isinstance(parts, bytearray):
+        return (struct_type * (len(parts) // N.ctypes.sizeof(struct_type))).from_buffer(parts)
     return (struct_type * max(1, len(parts))).from_buffer_copy(b"".join(parts) or bytes(N.ctypes.sizeof(struct_type)))
+
+
+def _count(struct_, parts) -> int:
+    return len(parts) // struct_.size if isinstance(parts, bytearray) else len(parts)
 
 
 def _per_tensor(x, n: int, what: str) -> list:
@@ -72,33 +78,32 @@ def _lists(**named):
     return list(out.values())
 
 
-def _check(ts, dtype, dev, what, shapes=None, distinct=True) -> list:
-    """Data pointers of ``ts`` after checking them (whole-list comparisons: a call may bring
-    hundreds of tensors, and the checks are most of its host time)."""
+# what a list's tensors have to be like (host_records.cpp)
+_ANY, _SAME_SHAPE, _FLAT_BLOCKS, _MATRIX_BLOCKS = 0, 1, 2, 3
+
+
+def _expected_shape(like, mode):
+    if mode == _SAME_SHAPE:
+        return tuple(like.shape)
+    runs, n = _runs(like.shape, mode == _MATRIX_BLOCKS)
+    return (runs, _blocks(n)) if mode == _MATRIX_BLOCKS else (_blocks(n),)
+
+
+def _pointers(rec, offset, stride, ts, dtype, dev, what, like=None, mode=_ANY, distinct=True) -> None:
+    """Checks the tensors and writes their pointers into the records at ``offset``."""
     index = dev.index if dev.index is not None else -1  # -1: the CPU
-    if not (set(map(_dtype_of, ts)) == {dtype} and set(map(_device_index, ts)) == {index} and all(map(_contiguous, ts))
-            and (shapes is None or list(map(_shape_of, ts)) == shapes)):
-        for i, t in enumerate(ts):
-            if t.dtype is not dtype:
-                raise TypeError(f"{what}[{i}] must be {dtype}, got {t.dtype}")
-            if t.device != dev:
-                raise RuntimeError(f"{what}[{i}] is on {t.device}, expected {dev}")
-            if not t.is_contiguous():
-                raise ValueError(f"{what}[{i}] must be contiguous")
-            if shapes is not None and t.shape != shapes[i]:
-                raise ValueError(f"{what}[{i}] must have shape {tuple(shapes[i])}, got {tuple(t.shape)}")
-        raise RuntimeError(f"{what}: unsupported tensors")
-    ptrs = list(map(_pointer, ts))
-    if distinct and len(set(ptrs)) != len(ptrs):
-        seen = [p for p, t in zip(ptrs, ts) if t.numel()]  # empty tensors may share an address
-        if len(set(seen)) != len(seen):
-            raise ValueError(f"{what}: the same tensor is given twice")
-    return ptrs
-
-
-_dtype_of, _shape_of = attrgetter("dtype"), attrgetter("shape")
-_device_index, _contiguous = torch.Tensor.get_device, torch.Tensor.is_contiguous
-_pointer, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
+    if N.host().pointers(rec, offset, stride, ts, dtype, index, like, mode, distinct):
+        return
+    for i, t in enumerate(ts):
+        if t.dtype is not dtype:
+            raise TypeError(f"{what}[{i}] must be {dtype}, got {t.dtype}")
+        if t.device != dev:
+            raise RuntimeError(f"{what}[{i}] is on {t.device}, expected {dev}")
+        if t.layout is not torch.strided or not t.is_contiguous():
+            raise ValueError(f"{what}[{i}] must be contiguous")
+        if mode != _ANY and tuple(t.shape) != _expected_shape(like[i], mode):
+            raise ValueError(f"{what}[{i}] must have shape {_expected_shape(like[i], mode)}, got {tuple(t.shape)}")
+    raise ValueError(f"{what}: the same tensor is given twice")
 
 
 def refuse_capture() -> None:
@@ -107,20 +112,19 @@ def refuse_capture() -> None:
                            "repeat at every replay: call it outside of graph capture")
 
 
+_here = nullcontext()
+
+
+def _on(dev):
+    """Makes ``dev`` the current device, which it mostly is already."""
+    return _here if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
 def _device(t) -> torch.device:
     if t.device.type != "cuda":
         raise RuntimeError(f"thorn_b200 runs its step on CUDA devices only; got a tensor on {t.device}")
     refuse_capture()
     return t.device
-
-
-def _strides(shape) -> tuple:
-    """Strides of a contiguous tensor."""
-    out, k = [1], 1
-    for d in reversed(shape[1:]):
-        k *= max(1, d)
-        out.append(k)
-    return tuple(reversed(out))
 
 
 @lru_cache(maxsize=4096)
@@ -151,7 +155,7 @@ def adam_record(p, g, w, m, v, ms, vs, numel, seed, lr, bc1, bc2, degenerate) ->
 def launch_adam(records, p_dtype, eight: bool, betas, weight_decay: float, eps: float, stream) -> None:
     lib = N.load()
     fn = lib.thorn_adamw8_multi if eight else lib.thorn_adamw_master_multi
-    N.check(fn(_records(N.AdamStateTensor, records), len(records), N.dtype_code(p_dtype), float(betas[0]),
+    N.check(fn(_records(N.AdamStateTensor, records), _count(_ADAM, records), N.dtype_code(p_dtype), float(betas[0]),
                float(betas[1]), float(weight_decay), float(eps), stream),
             "adamw8_multi" if eight else "adamw_master_multi")
 
@@ -164,19 +168,24 @@ def launch_momentum8(items, p_dtype, x_dtype, beta: float, dev, stream) -> None:
     for (g, m, ms, x, B, R, C, ldx, seed), nb in zip(items, need):
         recs.append(_MOMENTUM.pack(g, m, ms, x, B, R, C, ldx, seed & _U64, at if nb else 0))
         at += nb
-    N.check(N.load().thorn_momentum8_multi(_records(N.Momentum8Tensor, recs), len(recs), N.dtype_code(p_dtype),
-                                           N.dtype_code(x_dtype), beta, stream), "momentum8_multi")
+    _momentum_call(recs, p_dtype, x_dtype, beta, stream)
+
+
+def _momentum_call(recs, p_dtype, x_dtype, beta: float, stream) -> None:
+    N.check(N.load().thorn_momentum8_multi(_records(N.Momentum8Tensor, recs), _count(_MOMENTUM, recs),
+                                           N.dtype_code(p_dtype), N.dtype_code(x_dtype), beta, stream),
+            "momentum8_multi")
 
 
 def launch_apply(items, u_dtype, p_dtype, weight_decay: float, stream) -> None:
-    """``items``: (U, p, w, row_scale, mat_stats pointers, batch, rows, cols, lr)."""
-    N.check(N.load().thorn_apply_master_multi(_records(N.ApplyMasterTensor, [_APPLY.pack(*it) for it in items]),
-                                              len(items), N.dtype_code(u_dtype), N.dtype_code(p_dtype),
+    """``items``: (U, p, w, row_scale, mat_stats pointers, batch, rows, cols, lr), or their records."""
+    recs = items if isinstance(items, bytearray) else [_APPLY.pack(*it) for it in items]
+    N.check(N.load().thorn_apply_master_multi(_records(N.ApplyMasterTensor, recs), _count(_APPLY, recs),
+                                              N.dtype_code(u_dtype), N.dtype_code(p_dtype),
                                               float(weight_decay), stream), "apply_master_multi")
 
 
 # ------------------------------------------------------------------------------------- operators
-@torch.no_grad()
 def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor],
            variances: Sequence[torch.Tensor], *, step: Union[int, Sequence[int]],
            lr: Union[float, Sequence[float]], betas=(0.9, 0.95), eps: float = 0.0, weight_decay: float = 0.1,
@@ -204,56 +213,58 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
     dev, pdt, sdt = _device(params[0]), params[0].dtype, moments[0].dtype
     N.dtype_code(pdt)
     eight = sdt is CODES
-    steps, lrs = _per_tensor(step, n, "step"), _per_tensor(lr, n, "lr")
+    steps = _per_tensor(step, n, "step")
+    lrs = _per_tensor(lr, n, "lr")
     if min(steps) < 1:
         raise ValueError("step counts from 1")
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
         raise ValueError(f"betas must be in [0, 1), got {tuple(betas)}")
-    shapes = list(map(_shape_of, params))
-    pp = _check(params, pdt, dev, "params")
-    gp = _check(grads, pdt, dev, "grads", shapes, distinct=False)
-    mp = _check(moments, sdt, dev, "moments", shapes)
-    vp = _check(variances, sdt, dev, "variances", shapes)
-    numels = list(map(_numel, params))
-    wp = msp = vsp = repeat(0)
+    size = _ADAM.size
+    rec = bytearray(size * n)
+    _pointers(rec, 0, size, params, pdt, dev, "params")
+    _pointers(rec, 8, size, grads, pdt, dev, "grads", params, _SAME_SHAPE, distinct=False)
     if masters is not None:
         if pdt not in _HALF:
             raise TypeError(f"masters are fp32 copies of 16-bit parameters, got {pdt} parameters")
-        wp = _check(masters, torch.float32, dev, "masters", shapes)
+        _pointers(rec, 16, size, masters, torch.float32, dev, "masters", params, _SAME_SHAPE)
+    _pointers(rec, 24, size, moments, sdt, dev, "moments", params, _SAME_SHAPE)
+    _pointers(rec, 32, size, variances, sdt, dev, "variances", params, _SAME_SHAPE)
+    host = N.host()
     if eight:
         if ms is None or vs is None or seeds is None:
             raise ValueError("8-bit moments need moment_scales, variance_scales and seeds")
-        blocks = [(-(-k // BLOCK),) for k in numels]
-        msp = _check(ms, SCALES, dev, "moment_scales", blocks)
-        vsp = _check(vs, SCALES, dev, "variance_scales", blocks)
-        seeds = [x & _U64 for x in _per_tensor(seeds, n, "seeds")]
+        _pointers(rec, 40, size, ms, SCALES, dev, "moment_scales", params, _FLAT_BLOCKS)
+        _pointers(rec, 48, size, vs, SCALES, dev, "variance_scales", params, _FLAT_BLOCKS)
+        host.values(rec, 64, size, n, "Q", _per_tensor(seeds, n, "seeds"))
     else:
         if ms is not None or vs is not None:
             raise ValueError(f"scales are given with {sdt} moments")
         N.dtype_code(sdt)
         if masters is not None and sdt is not torch.float32:
             raise TypeError(f"masters need fp32 or 8-bit moments, got {sdt}")
-        seeds = repeat(0)
+    host.numels(rec, 56, size, params)
     scal = {}
     for t in set(steps):
-        scal[t] = (radam_rect(b2, t, rectify), 1 / (1 - b1 ** t), 1 / (1 - b2 ** t))
-    rects, bc1, bc2 = zip(*[scal[t] for t in steps])
-    rates = [x * r for x, r in zip(lrs, rects)]
-    first = [1 if r == 0.0 else 0 for r in rects]
-    with torch.cuda.device(dev):
+        rect = radam_rect(b2, t, rectify)
+        scal[t] = (rect, 1 / (1 - b1 ** t), 1 / (1 - b2 ** t), 1 if rect == 0.0 else 0)
+    columns = list(zip(*[scal[t] for t in steps])) if len(scal) > 1 else [[x] * n for x in scal[steps[0]]]
+    host.values(rec, 72, size, n, "f", [x * r for x, r in zip(lrs, columns[0])])
+    host.values(rec, 76, size, n, "f", list(columns[1]))
+    host.values(rec, 80, size, n, "f", list(columns[2]))
+    host.values(rec, 84, size, n, "i", list(columns[3]))
+    with _on(dev):
         stream = N.stream_of(dev)
         if eight or masters is not None:
-            launch_adam([_ADAM.pack(*r) for r in zip(pp, gp, wp, mp, vp, msp, vsp, numels, seeds, rates, bc1, bc2, first)],
-                        pdt, eight, (b1, b2), weight_decay, eps, stream)
+            launch_adam(rec, pdt, eight, (b1, b2), weight_decay, eps, stream)
         else:
-            recs = [N.AdamTensor(*r) for r in zip(pp, gp, mp, vp, numels, rates, bc1, bc2, first)]
+            recs = [N.AdamTensor(p, g, m, v, k, rate, c1, c2, deg) for p, g, _, m, v, _, _, k, _, rate, c1, c2, deg
+                    in _ADAM.iter_unpack(rec)]
             N.check(N.load().thorn_adamw_multi(N.array(N.AdamTensor, recs), n, N.dtype_code(pdt), N.dtype_code(sdt),
                                                float(b1), float(b2), float(weight_decay), float(eps), stream),
                     "adamw_multi")
 
 
-@torch.no_grad()
 def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], scales: Sequence[torch.Tensor], *,
               beta: float, seeds: Sequence[int], dtype: torch.dtype = torch.float16,
               out: Optional[Sequence[torch.Tensor]] = None) -> list:
@@ -277,33 +288,29 @@ def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], sc
     if not 0.0 <= beta < 1.0:
         raise ValueError(f"beta must be in [0, 1), got {beta}")
     seeds = _per_tensor(seeds, n, "seeds")
-    shapes = list(map(_shape_of, grads))
-    if min(map(len, shapes)) < 2:
-        raise ValueError("grads must be matrices or stacks of matrices")
-    views = [(prod(s[:-2]), s[-2], s[-1]) for s in shapes]
-    gp = _check(grads, pdt, dev, "grads", distinct=False)
-    mp = _check(moments, CODES, dev, "moments", shapes)
-    sp = _check(scales, SCALES, dev, "scales", [(B, -(-R * C // BLOCK)) for B, R, C in views])
-    if out is None:  # views of one allocation, each starting on 16 bytes: 30 allocations cost more than the launch
-        starts, total = [], 0
-        for B, R, C in views:
-            starts.append(total)
-            total += (B * R * C + 7) // 8 * 8
-        flat = torch.empty(total, dtype=dtype, device=dev)
-        out = [flat.as_strided(s, _strides(s), a) for s, a in zip(shapes, starts)]
-        base = flat.data_ptr()
-        xp = [base + 2 * a for a in starts]
-    else:
-        xp = _check(out, dtype, dev, "out", shapes)
-    items = [(g, m, s, x, B, R, C, C, seed) for g, m, s, x, (B, R, C), seed in zip(gp, mp, sp, xp, views, seeds)
-             if B and R and C]
-    if items:
-        with torch.cuda.device(dev):
-            launch_momentum8(items, pdt, dtype, float(beta), dev, N.stream_of(dev))
+    size = _MOMENTUM.size
+    rec = bytearray(size * n)
+    host = N.host()
+    _pointers(rec, 0, size, grads, pdt, dev, "grads", distinct=False)
+    views = host.matrices(rec, 32, size, grads)
+    _pointers(rec, 8, size, moments, CODES, dev, "moments", grads, _SAME_SHAPE)
+    _pointers(rec, 16, size, scales, SCALES, dev, "scales", grads, _MATRIX_BLOCKS)
+    host.values(rec, 64, size, n, "Q", seeds)
+    need = [_momentum_scratch(*v) for v in views]
+    if out is None:  # views of one allocation, each starting on 16 bytes
+        out = host.views(torch.empty(sum((B * R * C + 7) // 8 * 8 for B, R, C in views), dtype=dtype, device=dev), grads)
+    _pointers(rec, 24, size, out, dtype, dev, "out", grads, _SAME_SHAPE)
+    scratch = torch.empty(max(16, sum(need)), dtype=torch.uint8, device=dev)
+    starts, at = [], scratch.data_ptr()
+    for k in need:
+        starts.append(at)
+        at += k
+    host.values(rec, 72, size, n, "Q", starts)
+    with _on(dev):
+        _momentum_call(rec, pdt, dtype, float(beta), N.stream_of(dev))
     return out
 
 
-@torch.no_grad()
 def apply_update_(params: Sequence[torch.Tensor], updates: Sequence[torch.Tensor], *,
                   masters: Sequence[torch.Tensor], lr: Union[float, Sequence[float]],
                   weight_decay: float = 0.1) -> None:
@@ -320,14 +327,18 @@ def apply_update_(params: Sequence[torch.Tensor], updates: Sequence[torch.Tensor
     if pdt not in _HALF or udt not in _HALF:
         raise TypeError(f"params and updates must be float16 or bfloat16, got {pdt} and {udt}")
     lrs = _per_tensor(lr, n, "lr")
-    shapes = list(map(_shape_of, params))
-    pp = _check(params, pdt, dev, "params")
-    up = _check(updates, udt, dev, "updates", shapes, distinct=False)
-    wp = _check(masters, torch.float32, dev, "masters", shapes)
-    items = [(u, p, w, 0, 0, 1, 1, k, x) for p, u, w, k, x in zip(pp, up, wp, map(_numel, params), lrs) if k]
-    if items:
-        with torch.cuda.device(dev):
-            launch_apply(items, udt, pdt, weight_decay, N.stream_of(dev))
+    size = _APPLY.size
+    rec = bytearray(size * n)
+    host = N.host()
+    _pointers(rec, 8, size, params, pdt, dev, "params")
+    _pointers(rec, 0, size, updates, udt, dev, "updates", params, _SAME_SHAPE, distinct=False)
+    _pointers(rec, 16, size, masters, torch.float32, dev, "masters", params, _SAME_SHAPE)
+    host.values(rec, 40, size, n, "Q", 1)  # batch, rows: one row of all elements
+    host.values(rec, 48, size, n, "Q", 1)
+    host.numels(rec, 56, size, params)
+    host.values(rec, 64, size, n, "f", lrs)
+    with _on(dev):
+        launch_apply(rec, udt, pdt, weight_decay, N.stream_of(dev))
 
 
 # ------------------------------------------------------------------------------------ 8-bit state
