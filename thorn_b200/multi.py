@@ -62,7 +62,7 @@ def _count(struct_, parts) -> int:
 def _per_tensor(x, n: int, what: str) -> list:
     if isinstance(x, (int, float)):
         return [x] * n
-    x = list(x)
+    x = x if type(x) is list else list(x)
     if len(x) != n:
         raise ValueError(f"{what}: {len(x)} values for {n} tensors")
     return x
@@ -70,7 +70,7 @@ def _per_tensor(x, n: int, what: str) -> list:
 
 def _lists(**named):
     """The given tensor lists as lists of one length."""
-    out = {k: None if v is None else list(v) for k, v in named.items()}
+    out = {k: v if v is None or type(v) is list else list(v) for k, v in named.items()}
     n = len(next(iter(out.values())))
     for k, v in out.items():
         if v is not None and len(v) != n:
@@ -146,6 +146,23 @@ def radam_rect(beta2: float, step: int, rectify: bool) -> float:
     return 1.0
 
 
+def _adam_scalars(steps, lrs, b1: float, b2: float, rectify: bool, n: int):
+    """lr * rect, the bias corrections and the degenerate flag: four numbers where step and rate
+    are one for all tensors, else four lists."""
+    def of(t):
+        rect = radam_rect(b2, t, rectify)
+        return rect, 1 / (1 - b1 ** t), 1 / (1 - b2 ** t), 1 if rect == 0.0 else 0
+
+    if isinstance(steps, int) and isinstance(lrs, (int, float)):
+        rect, c1, c2, first = of(steps)
+        return lrs * rect, c1, c2, first
+    steps = [steps] * n if isinstance(steps, int) else steps
+    lrs = [lrs] * n if isinstance(lrs, (int, float)) else lrs
+    known = {t: of(t) for t in set(steps)}
+    rects, c1, c2, first = zip(*[known[t] for t in steps])
+    return [x * r for x, r in zip(lrs, rects)], list(c1), list(c2), list(first)
+
+
 # ------------------------------------------------------------------ launches (checked arguments)
 def adam_record(p, g, w, m, v, ms, vs, numel, seed, lr, bc1, bc2, degenerate) -> bytes:
     """One thorn_adamw_state_tensor; pointers as integers, 0 for NULL."""
@@ -213,9 +230,9 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
     dev, pdt, sdt = _device(params[0]), params[0].dtype, moments[0].dtype
     N.dtype_code(pdt)
     eight = sdt is CODES
-    steps = _per_tensor(step, n, "step")
-    lrs = _per_tensor(lr, n, "lr")
-    if min(steps) < 1:
+    steps = step if isinstance(step, int) else _per_tensor(step, n, "step")
+    lrs = lr if isinstance(lr, (int, float)) else _per_tensor(lr, n, "lr")
+    if (steps if isinstance(steps, int) else min(steps)) < 1:
         raise ValueError("step counts from 1")
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
@@ -244,15 +261,8 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
         if masters is not None and sdt is not torch.float32:
             raise TypeError(f"masters need fp32 or 8-bit moments, got {sdt}")
     host.numels(rec, 56, size, params)
-    scal = {}
-    for t in set(steps):
-        rect = radam_rect(b2, t, rectify)
-        scal[t] = (rect, 1 / (1 - b1 ** t), 1 / (1 - b2 ** t), 1 if rect == 0.0 else 0)
-    columns = list(zip(*[scal[t] for t in steps])) if len(scal) > 1 else [[x] * n for x in scal[steps[0]]]
-    host.values(rec, 72, size, n, "f", [x * r for x, r in zip(lrs, columns[0])])
-    host.values(rec, 76, size, n, "f", list(columns[1]))
-    host.values(rec, 80, size, n, "f", list(columns[2]))
-    host.values(rec, 84, size, n, "i", list(columns[3]))
+    for at, kind, column in zip((72, 76, 80, 84), "fffi", _adam_scalars(steps, lrs, b1, b2, rectify, n)):
+        host.values(rec, at, size, n, kind, column)
     with _on(dev):
         stream = N.stream_of(dev)
         if eight or masters is not None:
