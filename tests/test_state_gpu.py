@@ -676,3 +676,33 @@ def test_functions_chained_as_one_step():
     assert torch.equal(b, p[1].detach()) and torch.equal(wb, opt.state[p[1]]["master"])
     moved = opt.state[p[0]]["master"] - w0
     assert C.rel_fro((wa - w0).cpu().numpy(), moved.cpu().numpy()) <= 2e-2
+
+
+def _separately_rounded(kind, m, v, g, beta, w):
+    """The new state in torch's fp32, one rounding per operation (the products with powers of
+    two are exact)."""
+    if kind == "momentum":
+        return m * beta + g, None
+    return m + (g - m) * w[0], v * beta + g * g * w[1]
+
+
+def test_state_codes_are_those_of_separate_fp32_operations():
+    """2^22 elements: the new scales are those of the fp32 state formed operation by operation,
+    and every code is one of its two neighbours: the upper one exactly where the fraction asks."""
+    import thorn_b200 as T
+
+    n = 1 << 22
+    torch.manual_seed(11)
+    g = (torch.randn(n, device="cuda") * 1e-3).bfloat16()
+    p = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    mc, ms = T.state8_write(torch.randn(n, device="cuda") * 3e-4 + 0.1 * g.float())
+    vc, vs = T.state8_write(torch.randn(n, device="cuda").square() * 1e-6, positive=True)
+    mat = [t.view(2048, 2048) for t in (g, mc.clone())] + [ms.clone().view(1, -1)]
+    m0, v0 = T.state8_read(mc, ms), T.state8_read(vc, vs)
+    m1, v1 = _separately_rounded("adam", m0, v0, g.float(), 0.95, (1 - 0.9, 1 - 0.95))
+    k1, _ = _separately_rounded("momentum", m0, None, g.float(), 0.95, None)
+    T.adamw_([p], [g], [mc], [vc], step=2, lr=1e-3, moment_scales=[ms], variance_scales=[vs], seeds=[5])
+    T.momentum_([mat[0]], [mat[1]], [mat[2]], beta=0.95, seeds=[5])
+    frac = R.fractions(n, 5)
+    for x, c, s, pos in ((m1, mc, ms, False), (v1, vc, vs, True), (k1, mat[1], mat[2], False)):
+        R.check_state(f64(x), np.zeros(n), u8(c), u8(s), frac, pos, "bits")

@@ -142,6 +142,9 @@ __device__ __forceinline__ f2 add(f2 a, f2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// A packed product and a packed sum may come out as one fma.  Where the product is to be
+// rounded for itself, as the definition of the state has it, the sum is written as an fma
+// by a one that the compiler does not see (an argument of the kernel).
 __device__ __forceinline__ f2 fma(f2 a, f2 b, f2 c) {
   f2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
@@ -378,7 +381,7 @@ struct StAdam {
   int vec;
 };
 struct StAdamScalars {
-  float w1, beta2, w2, wd;  // w1 = 1 - beta1, w2 = 1 - beta2, formed in double
+  float w1, beta2, w2, wd, one;  // w1 = 1 - beta1, w2 = 1 - beta2, formed in double
 };
 template <int CAP>
 struct StAdamArgs {
@@ -417,7 +420,7 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
                                            const AdamIn<P, S8, MASTER>& in, const Rounding& rnd, uint32_t step,
                                            uint32_t& mb, uint32_t& vb) {
   f2 g[4], m[4], v[4];
-  const f2 w1 = dup(sc.w1), w2 = dup(sc.w2);
+  const f2 w1 = dup(sc.w1), w2 = dup(sc.w2), one = dup(sc.one);
   values(in.g, g);
   if constexpr (S8) {
     decode8(in.m, m);
@@ -427,7 +430,7 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       m[k] = fma(m[k], ms, mul(fma(m[k], neg, g[k]), w1));
-      v[k] = add(mul(v[k], vs), mul(mul(g[k], g[k]), w2));
+      v[k] = fma(mul(v[k], vs), one, mul(mul(g[k], g[k]), w2));
     }
     uint32_t top = top16(m) | (top16(v) << 16);
 #pragma unroll
@@ -457,8 +460,8 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
     const f2 b2 = dup(sc.beta2), neg = dup(-1.f);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      m[k] = add(m[k], mul(fma(m[k], neg, g[k]), w1));
-      v[k] = add(mul(v[k], b2), mul(mul(g[k], g[k]), w2));
+      m[k] = fma(m[k], one, mul(fma(m[k], neg, g[k]), w1));
+      v[k] = fma(mul(v[k], b2), one, mul(mul(g[k], g[k]), w2));
     }
     store8<FULL>((float*)e.m + i0, m, n);
     store8<FULL>((float*)e.v + i0, v, n);
@@ -579,7 +582,7 @@ struct StMomentum {
 template <int CAP>
 struct StMomentumArgs {
   StTable<StMomentum, CAP> tb;
-  float beta1;
+  float beta1, one;
 };
 
 // One matrix of a tensor.
@@ -597,13 +600,13 @@ __device__ __forceinline__ StMatrix<P> matrix_of(const StMomentum& e, int64_t b)
 // Momentum of one thread's 8 elements, mb as above; u = g + beta1 m from the rounded m.
 template <bool FULL, class P>
 __device__ __forceinline__ void momentum_step8(const StMatrix<P>& t, int64_t i0, int n, const Raw8<P>& graw, uint2 c,
-                                               uint32_t& mb, float beta1, const Rounding& rnd, uint32_t step, f2* u) {
+                                               uint32_t& mb, float beta1, float onef, const Rounding& rnd, uint32_t step, f2* u) {
   f2 g[4], m[4];
   values(graw, g);
   decode8(c, m);
-  const f2 s = dup(scale_value(mb) * beta1);
+  const f2 s = dup(scale_value(mb) * beta1), one = dup(onef);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) m[k] = add(mul(m[k], s), g[k]);
+  for (int k = 0; k < 4; ++k) m[k] = fma(mul(m[k], s), one, g[k]);
   uint32_t top = top16(m);
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -647,7 +650,7 @@ __device__ __forceinline__ float inverse_norm(float sumsq) { return 1.f / (sqrtf
 
 // Momentum of one chunk by the block; returns this thread's sum of squares of u.
 template <class P>
-__device__ __forceinline__ float momentum_chunk(const StMomentum& e, float beta1, int64_t b, int64_t chunk) {
+__device__ __forceinline__ float momentum_chunk(const StMomentum& e, float beta1, float onef, int64_t b, int64_t chunk) {
   const int64_t base = chunk * kStChunk;
   const int64_t seg = base + (threadIdx.x >> 5) * kStSeg, i0 = seg + (threadIdx.x & 31) * 8, blk = seg >> 7;
   const StMatrix<P> t = matrix_of<P>(e, b);
@@ -666,7 +669,7 @@ __device__ __forceinline__ float momentum_chunk(const StMomentum& e, float beta1
 #pragma unroll
     for (int it = 0; it < kStIter; ++it) {
       uint32_t mb = seg_byte(ms, it);
-      momentum_step8<true>(t, i0 + it * 256, 8, g[it], c[it], mb, beta1, rnd, it * 64, u);
+      momentum_step8<true>(t, i0 + it * 256, 8, g[it], c[it], mb, beta1, onef, rnd, it * 64, u);
 #pragma unroll
       for (int k = 0; k < 4; ++k) sq = fma(u[k], u[k], sq);
       out = put_byte(out, mb, it);
@@ -680,7 +683,7 @@ __device__ __forceinline__ float momentum_chunk(const StMomentum& e, float beta1
       Raw8<P> g;
       load_raw<false>(t.g + i, n, g);
       uint32_t mb = i < e.run ? t.ms[i >> 7] : 0u;
-      momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, beta1, rnd, it * 64, u);
+      momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, beta1, onef, rnd, it * 64, u);
 #pragma unroll
       for (int k = 0; k < 4; ++k) sq = fma(u[k], u[k], sq);
       if (i < e.run && (threadIdx.x & 15) == 0) t.ms[i >> 7] = (uint8_t)mb;
@@ -701,7 +704,7 @@ __global__ void __launch_bounds__(kStThreads, 6) momentum8_kernel(const __grid_c
   const StMomentum& e = a.tb.t[ti];
   const int64_t local = blockIdx.x - a.tb.start[ti];
   const int64_t b = local / e.chunks;
-  const float sq = momentum_chunk<P>(e, a.beta1, b, local - b * e.chunks);
+  const float sq = momentum_chunk<P>(e, a.beta1, a.one, b, local - b * e.chunks);
   if (e.x != nullptr) {
     const float tot = block_sum(sq, red);
     if (threadIdx.x == 0) e.part[local] = tot;
@@ -730,7 +733,7 @@ __global__ void __launch_bounds__(kStThreads) momentum8_small_kernel(const __gri
     Raw8<P> g;
     load_raw<false>(t.g + i, n, g);
     uint32_t mb = i < e.run ? t.ms[i >> 7] : 0u;
-    momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, a.beta1, rnd, it * 64, u[it]);
+    momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, a.beta1, a.one, rnd, it * 64, u[it]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) sq = fma(u[it][k], u[it][k], sq);
     if (i < e.run && (threadIdx.x & 15) == 0) t.ms[i >> 7] = (uint8_t)mb;
@@ -961,7 +964,7 @@ static int adam_launch(const thorn_adamw_state_tensor* ts, int n, const StAdamSc
 using namespace thorn;
 
 static StAdamScalars adam_scalars(double beta1, double beta2, float wd) {
-  return StAdamScalars{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), wd};
+  return StAdamScalars{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), wd, 1.f};
 }
 
 extern "C" int thorn_adamw8_multi(const thorn_adamw_state_tensor* ts, int n, int p_dtype, double beta1, double beta2,
@@ -1011,6 +1014,7 @@ static int momentum_launch(const thorn_momentum8_tensor* ts, int n, float beta1,
     StMomentumArgs<kStCap> a;
     a.tb = tb;
     a.beta1 = beta1;
+    a.one = 1.f;
     return a;
   };
   auto entry = [](const thorn_momentum8_tensor& t) {
