@@ -561,9 +561,8 @@ __global__ void __launch_bounds__(kStThreads, S8 && !MASTER ? 4 : 3)
 // ===========================================================================
 // momentum in 8 bits and the Newton-Schulz input
 // ===========================================================================
-// Matrices of one tensor, as one launch sees them.  Three forms by the matrix's length: up to
-// kStSeg elements a warp holds a whole matrix, up to kStChunk a block does; both then write
-// the input from registers.  Longer matrices take two readings: the momentum leaves one partial
+// Matrices of one tensor, as one launch sees them.  Two forms by the matrix's length: up to
+// kStChunk elements a group of lanes holds a whole matrix and writes the input from registers.  Longer matrices take two readings: the momentum leaves one partial
 // sum of squares per chunk, and the input reads g and the new codes again.
 struct StMomentum {
   const void* g;
@@ -711,43 +710,74 @@ __global__ void __launch_bounds__(kStThreads, 6) momentum8_kernel(const __grid_c
   }
 }
 
-// Matrices that a warp (WARP) or a block holds: momentum, norm and input at once.
-template <class P, class X, bool WARP, int CAP>
-__global__ void __launch_bounds__(kStThreads) momentum8_small_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
-  __shared__ float red[32];
-  const int ti = st_find(a.tb, blockIdx.x);
-  const StMomentum& e = a.tb.t[ti];
-  const int64_t local = blockIdx.x - a.tb.start[ti];
-  const int warp = threadIdx.x >> 5;
-  const int64_t b = WARP ? local * (kStThreads / 32) + warp : local;
-  if (WARP && b >= e.batch) return;  // whole warps, and no block-wide step in this form
-  const int64_t seg = WARP ? 0 : warp * kStSeg, i0 = seg + (threadIdx.x & 31) * 8;
-  const StMatrix<P> t = matrix_of<P>(e, b);
-  const Rounding rnd(i0, e.key, (uint32_t)b);
-  f2 sq = dup(0.f), u[kStIter][4];
+// Matrices that LANES lanes hold in IT times 8 elements each: half a warp, a warp or a block
+// of them.  Momentum, norm and input at once; the lanes take 8 elements in turn, so that all
+// of them have work, and every load is issued before the first is used.
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float x, float* red) {
+  if constexpr (LANES == kStThreads) {
+    return block_sum(x, red);
+  } else {
 #pragma unroll
-  for (int it = 0; it < kStIter; ++it) {
-    if (seg + it * 256 >= e.run) break;
-    const int64_t i = i0 + it * 256;
-    const int n = elems8(i, e.run, e.vec);
-    Raw8<P> g;
-    load_raw<false>(t.g + i, n, g);
-    uint32_t mb = i < e.run ? t.ms[i >> 7] : 0u;
-    momentum_step8<false>(t, i, n, g, load_codes<false>(t.m + i, n), mb, a.beta1, a.one, rnd, it * 64, u[it]);
+    for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+  }
+}
+template <class P, class X, int LANES, int IT>
+__device__ __forceinline__ void momentum_small(const StMomentum& e, int64_t block, float beta1, float one, float* red) {
+  const int64_t first = block * (kStThreads / LANES) + threadIdx.x / LANES;
+  const bool live = first < e.batch;  // lanes without a matrix stay for the shuffles
+  const int64_t b = live ? first : 0, run = live ? e.run : 0;
+  const int64_t i0 = (threadIdx.x % LANES) * 8;
+  const StMatrix<P> t = matrix_of<P>(e, b);
+  Raw8<P> g[IT];
+  uint2 c[IT];
+  uint32_t mb[IT];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int64_t i = i0 + it * (LANES * 8);
+    const int n = elems8(i, run, e.vec);
+    load_raw<false>(t.g + i, n, g[it]);
+    c[it] = load_codes<false>(t.m + i, n);
+    mb[it] = i < run ? t.ms[i >> 7] : 0u;
+  }
+  const Rounding rnd(i0, e.key, (uint32_t)b);
+  f2 sq = dup(0.f), u[IT][4];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int64_t i = i0 + it * (LANES * 8);
+    momentum_step8<false>(t, i, elems8(i, run, e.vec), g[it], c[it], mb[it], beta1, one, rnd, it * (LANES * 2), u[it]);
 #pragma unroll
     for (int k = 0; k < 4; ++k) sq = fma(u[it][k], u[it][k], sq);
-    if (i < e.run && (threadIdx.x & 15) == 0) t.ms[i >> 7] = (uint8_t)mb;
+    if (i < run && (threadIdx.x & 15) == 0) t.ms[i >> 7] = (uint8_t)mb[it];
   }
   float s0, s1;
   unpack_f2(sq, s0, s1);
-  const float inv = inverse_norm(WARP ? warp_sum(s0 + s1) : block_sum(s0 + s1, red));
+  const float inv = inverse_norm(lanes_sum<LANES>(s0 + s1, red));
   X* xb = (X*)e.x + b * (e.run / e.cols) * e.ldx;
 #pragma unroll
-  for (int it = 0; it < kStIter; ++it) {
-    const int64_t i = i0 + it * 256;
-    if (i >= e.run) break;
-    store_input8<false>(e, xb, i, elems8(i, e.run, e.vec), u[it], inv);
+  for (int it = 0; it < IT; ++it) {
+    const int64_t i = i0 + it * (LANES * 8);
+    if (i < run) store_input8<false>(e, xb, i, elems8(i, run, e.vec), u[it], inv);
   }
+}
+
+// Lanes that hold a matrix of up to kStChunk elements.
+__host__ __device__ inline int small_lanes(int64_t run) { return run <= 128 ? 16 : (run <= 1024 ? 32 : kStThreads); }
+
+// One launch for all lengths: the 30 tensors of a small convolutional model took 15.2 us,
+// 19.5 with the lengths that need one turn in a launch of their own (five blocks per SM) and
+// 23.5 with a launch per form; 60000 matrices of 8 x 8 took 18.7 us against 16.5.
+template <class P, class X, int CAP>
+__global__ void __launch_bounds__(kStThreads, 3) momentum8_small_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
+  __shared__ float red[32];
+  const int ti = st_find(a.tb, blockIdx.x);
+  const StMomentum& e = a.tb.t[ti];
+  const int64_t block = blockIdx.x - a.tb.start[ti];
+  const int lanes = small_lanes(e.run);
+  if (lanes == 16) momentum_small<P, X, 16, 1>(e, block, a.beta1, a.one, red);
+  else if (lanes == 32) momentum_small<P, X, 32, 4>(e, block, a.beta1, a.one, red);
+  else momentum_small<P, X, kStThreads, 4>(e, block, a.beta1, a.one, red);
 }
 
 // Partials that an input block sums by itself; the norm of a longer matrix is formed once,
@@ -1038,27 +1068,16 @@ static int momentum_launch(const thorn_momentum8_tensor* ts, int n, float beta1,
     return e;
   };
   auto live = [](const thorn_momentum8_tensor& t) { return st_elems(t.batch, t.rows, t.cols) > 0; };
+  // matrices that half a warp, a warp or a block holds
   int rc = st_launch<StMomentum, kStCap>(
       ts, n,
       [&](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t {
-        if (!live(t) || !t.x || t.rows * t.cols > kStSeg) return 0;
+        const int64_t run = t.rows * t.cols;
+        if (!live(t) || !t.x || run > kStChunk) return 0;
         e = entry(t);
-        return st_cdiv(t.batch, kStThreads / 32);
+        return st_cdiv(t.batch, kStThreads / small_lanes(run));
       },
-      [&](const Table& tb, unsigned nb) {
-        momentum8_small_kernel<P, X, true, kStCap><<<nb, kStThreads, 0, st>>>(args(tb));
-      });
-  if (rc) return rc;
-  rc = st_launch<StMomentum, kStCap>(
-      ts, n,
-      [&](const thorn_momentum8_tensor& t, StMomentum& e) -> int64_t {
-        if (!live(t) || !t.x || t.rows * t.cols <= kStSeg || t.rows * t.cols > kStChunk) return 0;
-        e = entry(t);
-        return t.batch;
-      },
-      [&](const Table& tb, unsigned nb) {
-        momentum8_small_kernel<P, X, false, kStCap><<<nb, kStThreads, 0, st>>>(args(tb));
-      });
+      [&](const Table& tb, unsigned nb) { momentum8_small_kernel<P, X, kStCap><<<nb, kStThreads, 0, st>>>(args(tb)); });
   if (rc) return rc;
   // momentum only, or longer than a block holds
   auto is_long = [&](const thorn_momentum8_tensor& t) { return live(t) && (!t.x || t.rows * t.cols > kStChunk); };
