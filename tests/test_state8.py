@@ -79,11 +79,11 @@ def test_prototypes_match_header():
 
 
 def test_scratch_bytes(lib):
-    # for matrices longer than 8192 elements: an fp32 sum per 8192 elements and one per matrix,
+    # for matrices longer than 4096 elements: an fp32 sum per 4096 elements and one per matrix,
     # padded to 16 bytes
-    assert lib.thorn_momentum8_scratch_bytes(7, 64, 128) == 0
+    assert lib.thorn_momentum8_scratch_bytes(7, 32, 128) == 0
     assert lib.thorn_momentum8_scratch_bytes(3, 65, 128) == 48
-    assert lib.thorn_momentum8_scratch_bytes(5, 128, 128) == 64
+    assert lib.thorn_momentum8_scratch_bytes(5, 128, 128) == 112
     assert lib.thorn_momentum8_scratch_bytes(0, 8, 8) == 0
     assert lib.thorn_momentum8_scratch_bytes(1, 1 << 40, 1 << 40) == 0  # over the size limit
 

@@ -23,8 +23,8 @@ pytestmark = pytest.mark.gpu
 E = 2.0 ** -24
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
-# lengths around the vector (8), the block (128), an iteration (2048) and a chunk (8192)
-LENGTHS = [1, 7, 8, 127, 128, 129, 2047, 2049, 8191, 8193, 20011]
+# lengths around the vector (8), the block (128), a warp's segment (1024) and a chunk (4096)
+LENGTHS = [1, 7, 8, 127, 128, 129, 1023, 1025, 2047, 4095, 4097, 8191, 8193, 20011]
 
 
 def f64(t):
@@ -303,8 +303,8 @@ def test_momentum_matches_float64(dtype, xdt):
     longer than a chunk, an empty one; two steps."""
     import thorn_b200 as T
 
-    shapes = [(1, 1), (2, 3), (8, 16), (5, 7, 9), (4, 6, 8), (2, 3, 5, 13), (129, 127), (65, 128), (3, 65, 200),
-              (0, 4), (130, 513)]
+    shapes = [(1, 1), (2, 3), (8, 16), (5, 7, 9), (70, 6, 8), (2, 3, 5, 13), (9, 15, 17), (9, 30, 30), (3, 40, 40),
+              (2, 64, 64), (129, 127), (65, 128), (3, 65, 200), (0, 4), (130, 513)]
     g, m, s = make_matrices(shapes, dtype)
     for step in range(2):
         before = [np.concatenate([R.read(c, b) for c, b in zip(u8(t).reshape(int(np.prod(t.shape[:-2])), -1),
@@ -317,6 +317,31 @@ def test_momentum_matches_float64(dtype, xdt):
             assert x[i].shape == g[i].shape and x[i].dtype is xdt
             if g[i].numel():
                 check_momentum(g[i], before[i], m[i], s[i], x[i], 0.95, seeds[i], xdt)
+
+
+@pytest.mark.parametrize("shape", [(20, 7, 9), (9, 13, 20), (5, 30, 30), (3, 50, 70), (2, 130, 130), (1, 700, 1101)])
+def test_momentum_with_padded_rows(shape):
+    """Rows of a longer leading dimension (the Newton-Schulz operand's) hold what the plain
+    layout holds, and the padding stays as it was."""
+    import thorn_b200 as T
+    from thorn_b200 import _native as N
+    from thorn_b200 import multi as M
+
+    B, R_, C_ = shape
+    g, m, s = make_matrices([shape], torch.bfloat16, seed=3)
+    m2, s2 = [t.clone() for t in m], [t.clone() for t in s]
+    x, = T.momentum_(g, m, s, beta=0.9, seeds=[4])
+    ld = int(N.load().thorn_ns_ld(C_)) + 8
+    X = torch.full((B, R_, ld), 9.0, dtype=torch.float16, device="cuda")
+    M.launch_momentum8([(g[0].data_ptr(), m2[0].data_ptr(), s2[0].data_ptr(), X.data_ptr(), B, R_, C_, ld, 4)],
+                       torch.bfloat16, torch.float16, 0.9, X.device, N.stream_of(X.device))
+    assert torch.equal(X[:, :, :C_], x) and bool((X[:, :, C_:] == 9).all())
+    assert np.array_equal(u8(m[0]), u8(m2[0])) and np.array_equal(u8(s[0]), u8(s2[0]))
+    # the momentum alone writes the same state
+    g3, m3, s3 = make_matrices([shape], torch.bfloat16, seed=3)
+    M.launch_momentum8([(g3[0].data_ptr(), m3[0].data_ptr(), s3[0].data_ptr(), 0, B, R_, C_, C_, 4)],
+                       torch.bfloat16, torch.float16, 0.9, X.device, N.stream_of(X.device))
+    assert np.array_equal(u8(m[0]), u8(m3[0])) and np.array_equal(u8(s[0]), u8(s3[0]))
 
 
 def test_momentum_large_and_reproducible():

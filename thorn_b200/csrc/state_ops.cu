@@ -9,15 +9,17 @@
 // change smaller than half a step (a second moment with beta2 near 1) is kept on average
 // instead of being lost at every step.
 //
-// Every kernel runs over flat chunks of 8192 elements with 8 consecutive elements per
-// thread, so 16 lanes hold one block of 128 and its maximum takes four shuffles.
+// Every kernel runs over flat chunks of 4096 elements with 8 consecutive elements per
+// thread, so 16 lanes hold one block of 128 and its maximum takes four shuffles.  Blocks of
+// 128 threads: with 256 (chunks of 8192) two 128256 x 4096 tensors took 1729 us instead of
+// 1711 and a stack of 4096 matrices of 64 x 64 took 45 us instead of 26.
 #include <math.h>
 
 #include "common.cuh"
 
 namespace thorn {
 
-constexpr int kStThreads = 256;
+constexpr int kStThreads = 128;
 constexpr int kStStep = kStThreads * 8;   // elements per block and iteration
 constexpr int kStChunk = 4 * kStStep;     // elements per thread block
 constexpr int kQBlock = 128;              // elements per 8-bit scale
@@ -500,12 +502,12 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
 
 // S8: moments in 8 bits, else fp32.  MASTER: the update is applied to fp32 master weights
 // and p receives their rounding.  The 8-bit form
-// without masters at four blocks per SM (64 registers): 1749 us for two 128256 x 4096
-// tensors, 1808 at the registers that it takes by itself, 1965 at three blocks and 1766 at
-// five, which spill.  The forms that move more bytes per element at three (80 registers): at
-// the 86 that it takes by itself 151936 x 1024 with masters took 450 us instead of 389.
+// without masters at eight blocks per SM (64 registers), the forms that move more bytes per
+// element at six (80).  In blocks of 256: two 128256 x 4096 tensors 1749 us at 64 registers,
+// 1808 at what it takes by itself, 1965 at 80 and 1766 at 48, which spill; 151936 x 1024 with
+// masters 389 at 80 and 450 at the 86 that it takes by itself.
 template <class P, bool S8, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kStThreads, S8 && !MASTER ? 4 : 3)
+__global__ void __launch_bounds__(kStThreads, S8 && !MASTER ? 8 : 6)
     adamw_state_kernel(const __grid_constant__ StAdamArgs<CAP> a) {
   const int ti = st_find(a.tb, blockIdx.x);
   const StAdam& e = a.tb.t[ti];
@@ -693,11 +695,11 @@ __device__ __forceinline__ float momentum_chunk(const StMomentum& e, float beta1
   return s0 + s1;
 }
 
-// The momentum pass.  Six blocks per SM (40 registers): more loads in flight than at the
+// The momentum pass.  Twelve blocks per SM (40 registers): more loads in flight than at the
 // registers that it takes by itself (decoder layer of 218 M elements, both passes: 322 us
 // against 339).
 template <class P, int CAP>
-__global__ void __launch_bounds__(kStThreads, 6) momentum8_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
+__global__ void __launch_bounds__(kStThreads, 12) momentum8_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
   __shared__ float red[32];
   const int ti = st_find(a.tb, blockIdx.x);
   const StMomentum& e = a.tb.t[ti];
@@ -769,7 +771,7 @@ __host__ __device__ inline int small_lanes(int64_t run) { return run <= 128 ? 16
 // 19.5 with the lengths that need one turn in a launch of their own (five blocks per SM) and
 // 23.5 with a launch per form; 60000 matrices of 8 x 8 took 18.7 us against 16.5.
 template <class P, class X, int CAP>
-__global__ void __launch_bounds__(kStThreads, 3) momentum8_small_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
+__global__ void __launch_bounds__(kStThreads, 6) momentum8_small_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
   __shared__ float red[32];
   const int ti = st_find(a.tb, blockIdx.x);
   const StMomentum& e = a.tb.t[ti];
@@ -782,7 +784,7 @@ __global__ void __launch_bounds__(kStThreads, 3) momentum8_small_kernel(const __
 
 // Partials that an input block sums by itself; the norm of a longer matrix is formed once,
 // by a launch between the passes.
-constexpr int kOwnSum = kStThreads;
+constexpr int kOwnSum = 4 * kStThreads;
 
 template <int CAP>
 __global__ void __launch_bounds__(1024) momentum8_norm_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
@@ -824,8 +826,17 @@ __global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __gri
     ms = load_seg_bytes(t.ms + blk);
   }
   float sumsq;
-  if (e.chunks <= kOwnSum) sumsq = block_sum(threadIdx.x < e.chunks ? e.part[b * e.chunks + threadIdx.x] : 0.f, red);
-  else sumsq = e.norm[b];
+  if (e.chunks <= kOwnSum) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < kOwnSum / kStThreads; ++k) {
+      const int i = k * kStThreads + threadIdx.x;
+      if (i < e.chunks) s += e.part[b * e.chunks + i];
+    }
+    sumsq = block_sum(s, red);
+  } else {
+    sumsq = e.norm[b];
+  }
   const float inv = inverse_norm(sumsq);
   f2 u[4], q[4];
   if (full) {
