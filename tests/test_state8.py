@@ -173,7 +173,7 @@ def test_cpu_tensors_are_refused():
 
 @pytest.mark.parametrize("change,error", [
     (dict(step=0), ValueError), (dict(step=[1]), ValueError), (dict(lr=[1.0]), ValueError),
-    (dict(betas=(0.9, 1.0)), ValueError), (dict(betas=(-0.1, 0.9)), ValueError),
+    (dict(eps=-1e-8), ValueError), (dict(betas=(0.9, 1.0)), ValueError), (dict(betas=(-0.1, 0.9)), ValueError),
     (dict(seeds=None), ValueError), (dict(seeds=[1]), ValueError), (dict(moment_scales=None), ValueError),
     (dict(grads=[]), ValueError),
     (dict(grads=[torch.zeros(3, 50), torch.zeros(3, 50)]), TypeError),

@@ -189,7 +189,7 @@ def test_zero_gradients_and_states():
     g = [torch.zeros_like(p[0])]
     (mc, ms), (vc, vs) = T.state8_zeros(p[0]), T.state8_zeros(p[0])
     kw = dict(lr=1e-2, weight_decay=0.0, moment_scales=[ms], variance_scales=[vs])
-    for eps in (0.0, 1e-8):
+    for eps in (0.0, 1e-8, 1e-40):
         T.adamw_(p, g, [mc], [vc], step=1, eps=eps, seeds=[3], **kw)
         assert bool((p[0] == 1).all()) and not u8(mc).any() and not u8(vc).any() and not u8(ms).any()
     g[0][5] = 1e-2

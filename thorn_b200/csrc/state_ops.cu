@@ -192,13 +192,14 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ uint32_t top16(const f2* v) {
+__device__ __forceinline__ uint32_t top_up(const f2* v) {
   float x[8];
 #pragma unroll
   for (int k = 0; k < 4; ++k) unpack_f2(v[k], x[2 * k], x[2 * k + 1]);
   const float t = max3_abs(max3_abs(x[0], x[1], x[2]), max3_abs(x[3], x[4], x[5]), max3_abs(x[6], x[7], x[7]));
-  return (__float_as_uint(t) + 0xffffu) >> 16;
+  return __float_as_uint(t) + 0xffffu;
 }
+__device__ __forceinline__ uint32_t top16(const f2* v) { return top_up(v) >> 16; }
 
 // Scale byte b of a block from its top16, the smallest power of two with max <= 448 * 2^k
 // (448 = 1.75 * 2^8 is the largest e4m3 value), and 2^(127 - b).  A block that is not finite
@@ -208,6 +209,19 @@ __device__ __forceinline__ uint32_t block_scale(uint32_t top, float& inverse) {
   const bool finite = top < 0x7f80u;
   inverse = __uint_as_float(finite ? (254u - b) << 23 : 0x7fc00000u);
   return finite ? b : 255u;
+}
+
+// block_scale of two blocks whose top16 lie in the halves of `top`, in 16-bit pairs.
+__device__ __forceinline__ void block_scales(uint32_t top, uint32_t& b0, uint32_t& b1, float& i0, float& i1) {
+  const uint32_t q = __vmaxu2(((top + 0x001f001fu) >> 7) & 0x01ff01ffu, 0x00080008u) - 0x00080008u;
+  b0 = q & 0xffffu;
+  b1 = q >> 16;
+  i0 = __uint_as_float((254u - b0) << 23);
+  i1 = __uint_as_float((254u - b1) << 23);
+  if ((top + 0x00800080u) & 0x80008000u) {  // one of them is not finite
+    if ((top & 0xffffu) >= 0x7f80u) b0 = 255u, i0 = __uint_as_float(0x7fc00000u);
+    if (top >= 0x7f800000u) b1 = 255u, i1 = __uint_as_float(0x7fc00000u);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -349,9 +363,16 @@ __device__ __forceinline__ f2 angle2(f2 y, f2 x2) {
   float t0, t1, q0, q1;
   unpack_f2(add(x2, dup(1.17549435e-38f)), q0, q1);
   unpack_f2(mul(y, pack_f2(rsqrt_approx(q0), rsqrt_approx(q1))), t0, t1);
-  const bool b0 = fabsf(t0) > 1.f, b1 = fabsf(t1) > 1.f;
-  const f2 s = pack_f2(b0 ? rcp_approx(-t0) : t0, b1 ? rcp_approx(-t1) : t1);
-  const f2 r = pack_f2(b0 ? copysignf(1.57079632679f, t0) : 0.f, b1 ? copysignf(1.57079632679f, t1) : 0.f);
+  float r0 = 0.f, r1 = 0.f;
+  if (fabsf(t0) > 1.f) {
+    r0 = copysignf(1.57079632679f, t0);
+    t0 = rcp_approx(-t0);
+  }
+  if (fabsf(t1) > 1.f) {
+    r1 = copysignf(1.57079632679f, t1);
+    t1 = rcp_approx(-t1);
+  }
+  const f2 s = pack_f2(t0, t1), r = pack_f2(r0, r1);
   const f2 z = mul(s, s);
   f2 p = dup(-0.0046932776f);
   p = fma(p, z, dup(0.02425241f));
@@ -434,12 +455,11 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
       m[k] = fma(m[k], ms, mul(fma(m[k], neg, g[k]), w1));
       v[k] = fma(mul(v[k], vs), one, mul(mul(g[k], g[k]), w2));
     }
-    uint32_t top = top16(m) | (top16(v) << 16);
+    uint32_t top = __byte_perm(top_up(m), top_up(v), 0x7632);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
     float mi1, vi1;
-    mb = block_scale(top & 0xffffu, mi1);
-    vb = block_scale(top >> 16, vi1);
+    block_scales(top, mb, vb, mi1, vi1);
     const f2 mi = dup(mi1), vi = dup(vi1);
     const uint32_t r0 = rnd.bits(step), r1 = rnd.bits(step + 1);
     f2 y[4];
@@ -501,13 +521,16 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
 }
 
 // S8: moments in 8 bits, else fp32.  MASTER: the update is applied to fp32 master weights
-// and p receives their rounding.  The 8-bit form
-// without masters at eight blocks per SM (64 registers), the forms that move more bytes per
-// element at six (80).  In blocks of 256: two 128256 x 4096 tensors 1749 us at 64 registers,
-// 1808 at what it takes by itself, 1965 at 80 and 1766 at 48, which spill; 151936 x 1024 with
-// masters 389 at 80 and 450 at the 86 that it takes by itself.
+// and p receives their rounding.
+//
+// The 8-bit form of 16-bit parameters without masters is bound by instruction issue where the power cap holds the
+// clock down (two 128256 x 4096 tensors: 1.74 ms at 1.97 GHz, 1.85 at the 1.69 that a second of
+// it runs at), the others by DRAM.  It takes nine blocks per SM (56 registers): 1845 us
+// against 1869 at eight; without reading one turn ahead 1909 at eight and 1936 at twelve.
+// The forms that move more bytes per element take six (80 registers): 389 us for 151936 x
+// 1024 with masters, and 450 at the 86 registers that they take by themselves.
 template <class P, bool S8, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kStThreads, S8 && !MASTER ? 8 : 6)
+__global__ void __launch_bounds__(kStThreads, S8 && !MASTER && sizeof(P) == 2 ? 9 : 6)
     adamw_state_kernel(const __grid_constant__ StAdamArgs<CAP> a) {
   const int ti = st_find(a.tb, blockIdx.x);
   const StAdam& e = a.tb.t[ti];
@@ -981,8 +1004,11 @@ static int adam_launch(const thorn_adamw_state_tensor* ts, int n, const StAdamSc
       [eps](const thorn_adamw_state_tensor& t, StAdam& e) -> int64_t {
         if ((t.w != nullptr) != MASTER) return 0;
         const double root = sqrt((double)t.bc2);
+        // a positive eps stays a normal number: the kernel takes zero for the arc tangent, and its
+        // reciprocal flushes subnormal arguments
+        const float eps_root = eps > 0.f ? fmaxf((float)(eps / root), 1.17549435e-38f) : 0.f;
         e = StAdam{t.p, t.g, (float*)t.w, t.m, t.v, (uint8_t*)t.m_scale, (uint8_t*)t.v_scale, t.numel,
-                   rounding_key(t.seed), t.lr, (float)(t.bc1 / root), (float)(eps / root), t.degenerate, 0};
+                   rounding_key(t.seed), t.lr, (float)(t.bc1 / root), eps_root, t.degenerate, 0};
         const bool mv = S8 ? aligned8(t.m) && aligned8(t.v) : aligned16(t.m) && aligned16(t.v);
         e.vec = mv && aligned16(t.g) && aligned16(t.p) && aligned16(t.w);
         return st_cdiv(t.numel, kStChunk);

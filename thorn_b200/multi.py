@@ -237,6 +237,8 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
         raise ValueError(f"betas must be in [0, 1), got {tuple(betas)}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
     size = _ADAM.size
     rec = bytearray(size * n)
     _pointers(rec, 0, size, params, pdt, dev, "params")
