@@ -99,6 +99,8 @@ PyObject* pointers(PyObject*, PyObject* args) {
     if (!rec.holds((Py_ssize_t)ts.size(), offset, stride, 8)) return bad_records();
     const at::ScalarType want = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
     std::vector<uint64_t> seen;
+    if (distinct) seen.reserve(ts.size());
+    bool ascending = true;
     for (size_t i = 0; i < ts.size(); ++i) {
       const at::Tensor& t = *ts[i];
       if (t.scalar_type() != want || t.layout() != at::kStrided || !t.is_contiguous()) Py_RETURN_FALSE;
@@ -106,10 +108,15 @@ PyObject* pointers(PyObject*, PyObject* args) {
       if (mode != kAny && !as_expected(t, *ls[i], mode)) Py_RETURN_FALSE;
       const uint64_t p = (uint64_t)(uintptr_t)t.data_ptr();
       rec.put(i, offset, stride, p);
-      if (distinct && numel_of(t) > 0) seen.push_back(p);  // empty tensors may share an address
+      if (distinct && numel_of(t) > 0) {  // empty tensors may share an address
+        ascending = ascending && (seen.empty() || seen.back() < p);
+        seen.push_back(p);
+      }
     }
-    std::sort(seen.begin(), seen.end());
-    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_FALSE;
+    if (!ascending) {
+      std::sort(seen.begin(), seen.end());
+      if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_FALSE;
+    }
   } catch (const std::exception& ex) {
     PyErr_SetString(PyExc_RuntimeError, ex.what());
     return nullptr;
@@ -161,51 +168,69 @@ PyObject* values(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-// matrices(records, offset, stride, tensors) -> list of (batch, rows, cols), also written as
-// int64 batch, rows, cols and leading dimension (= cols)
+// matrices(records, offset, stride, tensors, scratch function) -> (elements, bytes): writes
+// int64 batch, rows, cols and leading dimension (= cols); returns the elements of the outputs,
+// each padded to 8, and the bytes of all tensors' scratch.  The function is the library's
+// int64 (batch, rows, cols) -> bytes, as an address.
+using ScratchBytes = int64_t (*)(int64_t, int64_t, int64_t);
 PyObject* matrices(PyObject*, PyObject* args) {
   PyObject *buf, *list;
   Py_ssize_t offset, stride;
-  if (!PyArg_ParseTuple(args, "OnnO", &buf, &offset, &stride, &list)) return nullptr;
-  PyObject* out = nullptr;
+  unsigned long long fn;
+  if (!PyArg_ParseTuple(args, "OnnOK", &buf, &offset, &stride, &list, &fn)) return nullptr;
+  long long elems = 0, bytes = 0;
   try {
     std::vector<const at::Tensor*> ts;
     if (!tensors_of(list, ts)) return nullptr;
     Records rec(buf);
     if (!rec.ok) return nullptr;
     if (!rec.holds((Py_ssize_t)ts.size(), offset, stride, 32)) return bad_records();
-    out = PyList_New((Py_ssize_t)ts.size());
-    for (size_t i = 0; out && i < ts.size(); ++i) {
+    for (size_t i = 0; i < ts.size(); ++i) {
       const at::Tensor& t = *ts[i];
       const int64_t d = t.dim();
       if (d < 2) {
         PyErr_SetString(PyExc_ValueError, "grads must be matrices or stacks of matrices");
-        Py_CLEAR(out);
-        break;
+        return nullptr;
       }
       int64_t v[4] = {1, t.size(d - 2), t.size(d - 1), t.size(d - 1)};
       for (int64_t k = 0; k + 2 < d; ++k) v[0] *= t.size(k);
       for (int k = 0; k < 4; ++k) rec.put(i, offset + 8 * k, stride, v[k]);
-      PyObject* o = Py_BuildValue("(LLL)", (long long)v[0], (long long)v[1], (long long)v[2]);
-      if (!o) {
-        Py_CLEAR(out);
-        break;
-      }
-      PyList_SET_ITEM(out, (Py_ssize_t)i, o);
+      elems += (t.numel() + 7) / 8 * 8;
+      bytes += ((ScratchBytes)fn)(v[0], v[1], v[2]);
     }
   } catch (const std::exception& ex) {
-    Py_XDECREF(out);
     PyErr_SetString(PyExc_RuntimeError, ex.what());
     return nullptr;
   }
-  return out;
+  return Py_BuildValue("(LL)", elems, bytes);
 }
 
-// views(flat, like) -> list of tensors of the shapes of `like` that lie one after another in
-// `flat`, each starting at a multiple of 8 elements (the caller has allocated enough)
+// scratch(records, offset, at, stride, n, scratch function, base): writes each record's part of
+// the scratch at `base` at `at`, from the batch, rows and cols at `offset`
+PyObject* scratch(PyObject*, PyObject* args) {
+  PyObject* buf;
+  Py_ssize_t offset, at, stride, n;
+  unsigned long long fn, base;
+  if (!PyArg_ParseTuple(args, "OnnnnKK", &buf, &offset, &at, &stride, &n, &fn, &base)) return nullptr;
+  Records rec(buf);
+  if (!rec.ok) return nullptr;
+  if (!rec.holds(n, offset, stride, 24) || !rec.holds(n, at, stride, 8)) return bad_records();
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    int64_t v[3];
+    std::memcpy(v, (const char*)rec.view.buf + i * stride + offset, sizeof(v));
+    rec.put(i, at, stride, (uint64_t)base);
+    base += (uint64_t)((ScratchBytes)fn)(v[0], v[1], v[2]);
+  }
+  Py_RETURN_NONE;
+}
+
+// views(flat, like, records, offset, stride) -> list of tensors of the shapes of `like` that
+// lie one after another in `flat`, each starting at a multiple of 8 elements (the caller has
+// allocated enough); their pointers are written into the records
 PyObject* views(PyObject*, PyObject* args) {
-  PyObject *flat, *list;
-  if (!PyArg_ParseTuple(args, "OO", &flat, &list)) return nullptr;
+  PyObject *flat, *list, *buf;
+  Py_ssize_t offset, stride;
+  if (!PyArg_ParseTuple(args, "OOOnn", &flat, &list, &buf, &offset, &stride)) return nullptr;
   if (!THPVariable_Check(flat)) {
     PyErr_SetString(PyExc_TypeError, "expected a tensor");
     return nullptr;
@@ -214,6 +239,9 @@ PyObject* views(PyObject*, PyObject* args) {
   try {
     std::vector<const at::Tensor*> ts;
     if (!tensors_of(list, ts)) return nullptr;
+    Records rec(buf);
+    if (!rec.ok) return nullptr;
+    if (!rec.holds((Py_ssize_t)ts.size(), offset, stride, 8)) return bad_records();
     const at::Tensor& f = THPVariable_Unpack(flat);
     int64_t total = 0;
     for (const at::Tensor* t : ts) total += (t->numel() + 7) / 8 * 8;
@@ -222,6 +250,8 @@ PyObject* views(PyObject*, PyObject* args) {
       return nullptr;
     }
     at::AutoDispatchBelowAutograd no_autograd;  // plain buffers: no view tracking
+    const uint64_t base = (uint64_t)(uintptr_t)f.data_ptr();
+    const int64_t width = f.element_size();
     out = PyList_New((Py_ssize_t)ts.size());
     int64_t at = 0;
     std::vector<int64_t> strides;
@@ -235,6 +265,7 @@ PyObject* views(PyObject*, PyObject* args) {
         break;
       }
       PyList_SET_ITEM(out, (Py_ssize_t)i, o);
+      rec.put(i, offset, stride, base + (uint64_t)(at * width));
       at += (n + 7) / 8 * 8;
     }
   } catch (const std::exception& ex) {
@@ -250,6 +281,7 @@ PyMethodDef kMethods[] = {
     {"numels", numels, METH_VARARGS, "write element counts"},
     {"values", values, METH_VARARGS, "write scalars"},
     {"matrices", matrices, METH_VARARGS, "write batch, rows and columns"},
+    {"scratch", scratch, METH_VARARGS, "write scratch pointers"},
     {"views", views, METH_VARARGS, "views of one buffer"},
     {nullptr, nullptr, 0, nullptr},
 };

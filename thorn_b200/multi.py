@@ -120,6 +120,11 @@ def _on(dev):
     return _here if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+def _stream(dev) -> int:
+    """The current stream of ``dev``."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def _device(t) -> torch.device:
     if t.device.type != "cuda":
         raise RuntimeError(f"thorn_b200 runs its step on CUDA devices only; got a tensor on {t.device}")
@@ -130,6 +135,12 @@ def _device(t) -> torch.device:
 @lru_cache(maxsize=4096)
 def _momentum_scratch(B: int, R: int, C: int) -> int:
     return int(N.load().thorn_momentum8_scratch_bytes(B, R, C))
+
+
+@lru_cache(maxsize=None)
+def _scratch_fn() -> int:
+    """Address of thorn_momentum8_scratch_bytes."""
+    return N.ctypes.cast(N.load().thorn_momentum8_scratch_bytes, N.ctypes.c_void_p).value
 
 
 def _blocks(numel: int) -> int:
@@ -266,7 +277,7 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
     for at, kind, column in zip((72, 76, 80, 84), "fffi", _adam_scalars(steps, lrs, b1, b2, rectify, n)):
         host.values(rec, at, size, n, kind, column)
     with _on(dev):
-        stream = N.stream_of(dev)
+        stream = _stream(dev)
         if eight or masters is not None:
             launch_adam(rec, pdt, eight, (b1, b2), weight_decay, eps, stream)
         else:
@@ -304,22 +315,18 @@ def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], sc
     rec = bytearray(size * n)
     host = N.host()
     _pointers(rec, 0, size, grads, pdt, dev, "grads", distinct=False)
-    views = host.matrices(rec, 32, size, grads)
+    elems, need = host.matrices(rec, 32, size, grads, _scratch_fn())
     _pointers(rec, 8, size, moments, CODES, dev, "moments", grads, _SAME_SHAPE)
     _pointers(rec, 16, size, scales, SCALES, dev, "scales", grads, _MATRIX_BLOCKS)
     host.values(rec, 64, size, n, "Q", seeds)
-    need = [_momentum_scratch(*v) for v in views]
     if out is None:  # views of one allocation, each starting on 16 bytes
-        out = host.views(torch.empty(sum((B * R * C + 7) // 8 * 8 for B, R, C in views), dtype=dtype, device=dev), grads)
-    _pointers(rec, 24, size, out, dtype, dev, "out", grads, _SAME_SHAPE)
-    scratch = torch.empty(max(16, sum(need)), dtype=torch.uint8, device=dev)
-    starts, at = [], scratch.data_ptr()
-    for k in need:
-        starts.append(at)
-        at += k
-    host.values(rec, 72, size, n, "Q", starts)
+        out = host.views(torch.empty(elems, dtype=dtype, device=dev), grads, rec, 24, size)
+    else:
+        _pointers(rec, 24, size, out, dtype, dev, "out", grads, _SAME_SHAPE)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    host.scratch(rec, 32, 72, size, n, _scratch_fn(), 0 if scratch is None else scratch.data_ptr())
     with _on(dev):
-        _momentum_call(rec, pdt, dtype, float(beta), N.stream_of(dev))
+        _momentum_call(rec, pdt, dtype, float(beta), _stream(dev))
     return out
 
 
@@ -350,7 +357,7 @@ def apply_update_(params: Sequence[torch.Tensor], updates: Sequence[torch.Tensor
     host.numels(rec, 56, size, params)
     host.values(rec, 64, size, n, "f", lrs)
     with _on(dev):
-        launch_apply(rec, udt, pdt, weight_decay, N.stream_of(dev))
+        launch_apply(rec, udt, pdt, weight_decay, _stream(dev))
 
 
 # ------------------------------------------------------------------------------------ 8-bit state
