@@ -25,10 +25,10 @@ def _fold(a, b):
     return (t >> np.uint64(32)) ^ (t & np.uint64(M32))
 
 
-def fractions(n, seed, run=0):
-    """The rounding fraction in [0, 1) of each of n elements of run ``run``."""
+def fractions(n, seed, run=0, start=0):
+    """The rounding fraction in [0, 1) of n elements of run ``run`` from ``start`` (a multiple of 4)."""
     key = key_of(seed)
-    q = np.arange(-(-n // 4), dtype=np.uint64)
+    q = np.arange(-(-n // 4), dtype=np.uint64) + np.uint64(start // 4)
     a = ((q & np.uint64(M32)) * np.uint64(0x9E3779B9) + np.uint64(key & M32)) & np.uint64(M32)
     hi = ((q >> np.uint64(32)) + np.uint64(run)) & np.uint64(M32)
     x = _fold(a, a ^ np.uint64(key >> 32) ^ hi)

@@ -17,7 +17,7 @@ from thorn_b200 import multi as M
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-@pytest.fixture(scope="module")
+@pytest.fixture(scope="module", autouse=True)
 def lib():
     B.build()
     return N.load()

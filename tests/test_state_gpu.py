@@ -440,6 +440,72 @@ def test_other_stream_and_neighbours_untouched():
     assert bool((codes[:32] == 0x55).all()) and bool((codes[32 + n:] == 0x55).all())
 
 
+def test_offsets_beyond_32_bits():
+    """2^32 + 5000 elements: the tail is updated with the random numbers of its own place, and what
+    lies before it stays zero.  The tail starts inside a block."""
+    import thorn_b200 as T
+
+    n, tail = (1 << 32) + 5000, 4936
+    if torch.cuda.get_device_properties(0).total_memory < 60 << 30:
+        pytest.skip("needs 30 GB")
+    p = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    torch.manual_seed(12)
+    g[n - tail:] = (torch.randn(tail, device="cuda") * 1e-3).bfloat16()
+    (mc, ms), (vc, vs) = T.state8_zeros(p), T.state8_zeros(p)
+    T.adamw_([p], [g], [mc], [vc], step=1, lr=1e-2, weight_decay=0.0, moment_scales=[ms], variance_scales=[vs], seeds=[6])
+    at = (n - tail) // 128 * 128  # the block that the tail starts in
+    x = f64(g[at:])
+    frac = R.fractions(n - at, 6, start=at)
+    m2, v2 = 0.1 * x, 0.05 * x * x
+    R.check_state(m2, 5 * E * np.abs(x), u8(mc[at:]), u8(ms[at // 128:]), frac, False, "m")
+    R.check_state(v2, 5 * E * v2, u8(vc[at:]), u8(vs[at // 128:]), frac, True, "v")
+    assert bool((p[n - tail:][g[n - tail:] != 0] != 0).all())
+    assert int(torch.count_nonzero(mc[:at].view(torch.int64))) == 0 and int(torch.count_nonzero(p[:at].view(torch.int64))) == 0
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with its own tensors and scratch, give what they give alone."""
+    import thorn_b200 as T
+
+    shapes = [(300, 400), (6, 90, 70), (40, 30)]
+    want, got = [], []
+    for together in (False, True):
+        sets = [make_matrices(shapes, torch.bfloat16, seed=20 + k) for k in range(2)]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        out = [None, None]
+        for step in range(3):
+            for k in range(2):
+                g, m, s = sets[k]
+                with torch.cuda.stream(streams[k]):
+                    out[k] = T.momentum_(g, m, s, beta=0.9, seeds=[step, step + 10, step + 20])
+                if not together:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        (got if together else want).extend([u8(t).copy() for k in range(2) for t in out[k] + sets[k][1] + sets[k][2]])
+    for a, b in zip(want, got):
+        assert np.array_equal(a, b)
+
+
+def test_mixed_parameter_types_in_one_group():
+    """fp32, bf16 and fp16 parameters of one group with 8-bit state, a scalar and an empty one
+    among the AdamW ones."""
+    import thorn_b200 as T
+
+    for ortho, shapes in ((True, [(20, 30), (20, 30), (20, 30)]), (False, [(50,), (), (0,), (7, 9)])):
+        dts = [torch.float32, torch.bfloat16, torch.float16, torch.bfloat16][:len(shapes)]
+        p = [torch.nn.Parameter((torch.randn(s, device="cuda") * 0.02).to(d)) for s, d in zip(shapes, dts)]
+        before = [t.detach().clone() for t in p]
+        opt = T.THORN([{"orthogonalize": ortho, "params": p, "lr": 1e-2, "state_dtype": F8, "master_weights": True}])
+        for t in p:
+            t.grad = torch.ones_like(t) * 1e-3 + torch.arange(t.numel(), device="cuda").reshape(t.shape).to(t.dtype) * 1e-5
+        opt.step()
+        for t, b, d in zip(p, before, dts):
+            assert ("master" in opt.state[t]) == (d is not torch.float32)
+            assert bool(t.isfinite().all()) and (t.numel() == 0 or not torch.equal(t.detach(), b))
+
+
 def test_capture_is_refused():
     import thorn_b200 as T
 

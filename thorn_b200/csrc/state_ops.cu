@@ -293,6 +293,11 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint2 c, int n) {
   }
 }
 
+// i / cols, by the short division where it does
+__device__ __forceinline__ int64_t row_of(int64_t i, int64_t cols) {
+  return ((uint64_t)i | (uint64_t)cols) >> 32 ? i / cols : (int64_t)((uint32_t)i / (uint32_t)cols);
+}
+
 __device__ __forceinline__ int elems8(int64_t i, int64_t end, int vec) {
   return (int)max64(0, min64(8, end - i)) + (vec ? kVec : 0);
 }
@@ -659,7 +664,7 @@ __device__ __forceinline__ void store_input8(const StMomentum& e, X* xb, int64_t
     float v[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) unpack_f2(u[k], v[2 * k], v[2 * k + 1]);
-    int64_t r = i0 / e.cols, col = i0 - r * e.cols;
+    int64_t r = row_of(i0, e.cols), col = i0 - r * e.cols;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (k < (n & 15)) xb[r * e.ldx + col] = from_f<X>(v[k]);
@@ -927,20 +932,23 @@ __device__ __forceinline__ void apply_step8(const StApply& e, float wd, int64_t 
     unpack_f2(w[k], wv[2 * k], wv[2 * k + 1]);
   }
   if (e.row_scale != nullptr) {
-    int64_t r = i0 / e.cols, c = i0 - r * e.cols;
+    int64_t r = row_of(i0, e.cols), c = i0 - r * e.cols;
+    auto factor = [&](int64_t row) {
+      float s = e.row_scale[row];
+      if (e.mat_stats != nullptr) {
+        const float* st = e.mat_stats + 2 * row_of(row, e.rows);
+        s *= sqrtf(st[0]) / fmaxf(sqrtf(st[1]), kF32Eps);
+      }
+      return s;
+    };
+    float s = factor(r);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (FULL || k < (n & 15)) {
-        float s = e.row_scale[r];
-        if (e.mat_stats != nullptr) {
-          const int64_t b = r / e.rows;
-          s *= sqrtf(e.mat_stats[2 * b]) / fmaxf(sqrtf(e.mat_stats[2 * b + 1]), kF32Eps);
-        }
-        uv[k] *= s;
-      }
+      uv[k] *= s;  // past the end: zeros that are not stored
       if (++c == e.cols) {
         c = 0;
         ++r;
+        if (k < 7 && i0 + k + 1 < e.numel) s = factor(r);
       }
     }
   }

@@ -146,13 +146,7 @@ class GroupConfig:
 
     def rect(self, step) -> float:
         """RAdam rectification (thorn.py:782-798)."""
-        beta2 = self.betas[1]
-        if beta2 > 0.0:
-            rho_inf = 2 / (1 - beta2) - 1
-            rho = rho_inf - 2 * step * (beta2 ** step) / (1 - beta2 ** step)
-            r = ((rho - 4) * (rho - 2) * rho_inf / ((rho_inf - 4) * (rho_inf - 2) * rho)) ** 0.5 if rho > 4.0 else 0.0
-            return r ** float(self.rectify)
-        return 1.0
+        return multi.radam_rect(self.betas[1], step, self.rectify)
 
     def target_norm_(self, p: torch.Tensor) -> torch.Tensor:
         """thorn.py:597-612 (run once, at state creation)."""
