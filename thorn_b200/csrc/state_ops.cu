@@ -533,7 +533,8 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
 // it runs at), the others by DRAM.  It takes nine blocks per SM (56 registers): 1845 us
 // against 1869 at eight; without reading one turn ahead 1909 at eight and 1936 at twelve.
 // The forms that move more bytes per element take six (80 registers): 389 us for 151936 x
-// 1024 with masters, and 450 at the 86 registers that they take by themselves.
+// 1024 with masters, and 450 at the 86 registers that they take by themselves; the fp32 form
+// moves 28 bytes per element at the copy rate (659 us for that size).
 template <class P, bool S8, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kStThreads, S8 && !MASTER && sizeof(P) == 2 ? 9 : 6)
     adamw_state_kernel(const __grid_constant__ StAdamArgs<CAP> a) {
@@ -592,8 +593,9 @@ __global__ void __launch_bounds__(kStThreads, S8 && !MASTER && sizeof(P) == 2 ? 
 // momentum in 8 bits and the Newton-Schulz input
 // ===========================================================================
 // Matrices of one tensor, as one launch sees them.  Two forms by the matrix's length: up to
-// kStChunk elements a group of lanes holds a whole matrix and writes the input from registers.  Longer matrices take two readings: the momentum leaves one partial
-// sum of squares per chunk, and the input reads g and the new codes again.
+// kStChunk elements a group of lanes holds a whole matrix and writes the input from registers.
+// Longer matrices take two readings: the momentum leaves one partial sum of squares per chunk,
+// and the input reads g and the new codes again.
 struct StMomentum {
   const void* g;
   uint8_t* m;
@@ -629,7 +631,8 @@ __device__ __forceinline__ StMatrix<P> matrix_of(const StMomentum& e, int64_t b)
 // Momentum of one thread's 8 elements, mb as above; u = g + beta1 m from the rounded m.
 template <bool FULL, class P>
 __device__ __forceinline__ void momentum_step8(const StMatrix<P>& t, int64_t i0, int n, const Raw8<P>& graw, uint2 c,
-                                               uint32_t& mb, float beta1, float onef, const Rounding& rnd, uint32_t step, f2* u) {
+                                               uint32_t& mb, float beta1, float onef, const Rounding& rnd,
+                                               uint32_t step, f2* u) {
   f2 g[4], m[4];
   values(graw, g);
   decode8(c, m);
@@ -723,9 +726,10 @@ __device__ __forceinline__ float momentum_chunk(const StMomentum& e, float beta1
   return s0 + s1;
 }
 
-// The momentum pass.  Twelve blocks per SM (40 registers): more loads in flight than at the
-// registers that it takes by itself (decoder layer of 218 M elements, both passes: 322 us
-// against 339).
+// The momentum pass: 4 bytes per element with 16-bit gradients, 19 instructions, which keep
+// the issue slots near 80 % busy at 89 % of the copy rate (153 us for the 218 M elements of a
+// decoder layer).  Twelve blocks per SM (40 registers): more loads in flight than at the
+// registers that it takes by itself (both passes 322 us against 339).
 template <class P, int CAP>
 __global__ void __launch_bounds__(kStThreads, 12) momentum8_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
   __shared__ float red[32];
@@ -828,8 +832,8 @@ __global__ void __launch_bounds__(1024) momentum8_norm_kernel(const __grid_const
   if (threadIdx.x == 0) e.norm[b] = s;
 }
 
-// The input pass, from the last chunk to the first: what the momentum pass read and wrote
-// last is then still in L2.
+// The input pass: 5 bytes per element, bound by DRAM (152 us for 218 M elements).  From the
+// last chunk to the first: what the momentum pass read and wrote last is then still in L2.
 template <class P, class X, int CAP>
 __global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
   __shared__ float red[32];
@@ -898,6 +902,8 @@ __global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __gri
 // ===========================================================================
 // apply onto fp32 master weights
 // ===========================================================================
+// 12 bytes per element, bound by DRAM: 391 us for 218 M elements (6.7 TB/s); with the row and
+// matrix factors of a 14336 x 4096 matrix 116 us instead of 109.
 struct StApply {
   const void* U;
   void* p;
