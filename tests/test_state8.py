@@ -371,3 +371,51 @@ def test_state_layout_and_state_dict_round_trip():
                 assert w.dtype is v.dtype and torch.equal(w.view(torch.uint8), v.view(torch.uint8)), k
             else:
                 assert w == v
+
+
+# --------------------------------------------------------------------------- the host extension
+def test_host_extension_refuses_bad_arguments(lib):
+    h = N.host()
+    ts = [torch.zeros(3), torch.zeros(4, 5)]
+    f32 = torch.float32
+
+    def ptr(buf=None, offset=0, stride=16, t=ts, dtype=f32, device=-1, like=None, mode=0, distinct=True):
+        return h.pointers(bytearray(64) if buf is None else buf, offset, stride, t, dtype, device, like, mode, distinct)
+
+    buf = bytearray(64)
+    assert ptr(buf=buf, offset=8) is True
+    assert [int.from_bytes(buf[16 * i + 8:16 * i + 16], "little") for i in (0, 1)] == [t.data_ptr() for t in ts]
+    assert buf[:8] == bytes(8) and buf[32:] == bytes(32)
+    assert ptr(dtype=torch.float64) is False and ptr(device=0) is False
+    assert ptr(t=[ts[1].T]) is False and ptr(t=[ts[0], ts[0]]) is False and ptr(t=[ts[0], ts[0]], distinct=False) is True
+    assert ptr(t=[torch.zeros(0), torch.zeros(0)]) is True  # empty tensors may share an address
+    assert ptr(t=[ts[0].to_sparse()]) is False and ptr(t=[torch.zeros(3, device="meta")]) is False
+    assert ptr(like=ts, mode=1) is True and ptr(like=ts[::-1], mode=1) is False
+    a, b = torch.zeros(300), torch.zeros(2, 10, 30)
+    assert ptr(t=[torch.zeros(3), torch.zeros(5)], like=[a, b], mode=2) is True
+    assert ptr(t=[torch.zeros(2, 3)], like=[b], mode=3) is True and ptr(t=[torch.zeros(3)], like=[a], mode=3) is False
+    for bad, error in [(dict(t=tuple(ts)), TypeError), (dict(t=[1]), TypeError), (dict(dtype="float32"), TypeError),
+                       (dict(like=ts[:1], mode=1), ValueError), (dict(buf=bytearray(31)), ValueError),
+                       (dict(offset=-8), ValueError), (dict(offset=12), ValueError), (dict(buf=b"x" * 64), BufferError)]:
+        with pytest.raises(error):
+            ptr(**bad)
+    with pytest.raises(ValueError):
+        h.values(bytearray(16), 0, 8, 2, "f", [1.0])
+    with pytest.raises(ValueError):
+        h.values(bytearray(15), 0, 8, 2, "f", 1.0)
+    with pytest.raises(TypeError):
+        h.values(bytearray(16), 0, 8, 2, "f", ["x", "y"])
+    fn = M._scratch_fn()
+    with pytest.raises(ValueError, match="matrices"):
+        h.matrices(bytearray(64), 0, 64, [torch.zeros(3)], fn)
+    rec = bytearray(2 * 40)
+    assert h.matrices(rec, 0, 40, [torch.zeros(3, 65, 128), torch.zeros(5, 7)], fn) == (3 * 65 * 128 + 40, 48)
+    h.scratch(rec, 0, 32, 40, 2, fn, 4096)
+    assert [int.from_bytes(rec[40 * i + 32:40 * i + 40], "little") for i in (0, 1)] == [4096, 4096 + 48]
+    assert list(memoryview(rec)[:32].cast("q")) == [3, 65, 128, 128]
+    flat = torch.arange(80, dtype=torch.float16)
+    v = h.views(flat, [torch.zeros(3, 7), torch.zeros(2, 0, 4), torch.zeros(5, 9)], bytearray(48), 0, 16)
+    assert [tuple(x.shape) for x in v] == [(3, 7), (2, 0, 4), (5, 9)] and all(x.is_contiguous() for x in v)
+    assert v[2].data_ptr() == flat.data_ptr() + 2 * 24 and float(v[2][4, 8]) == 24 + 44
+    with pytest.raises(ValueError, match="short"):
+        h.views(flat, [torch.zeros(9, 9)], bytearray(16), 0, 16)
