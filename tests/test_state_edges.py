@@ -1,0 +1,62 @@
+"""Edges of the optimizer state on the CPU: saving and loading, refusals and host code.  The
+kernels' edges are in test_state_edges_gpu.py."""
+import pytest
+import torch
+
+from thorn_b200 import THORN
+from thorn_b200 import build as B
+from thorn_b200 import multi as M
+
+F8 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    B.build()
+
+
+def _with_state(groups):
+    """A THORN whose parameters' states are made and filled with numbers (the step itself needs a GPU)."""
+    opt = THORN(groups)
+    gen = torch.Generator().manual_seed(1)
+    for group in opt.param_groups:
+        for p in group["params"]:
+            p.grad = torch.zeros_like(p)
+            with pytest.raises(RuntimeError, match="CUDA devices only"):
+                opt.step(param=p)
+            for k, v in opt.state[p].items():
+                if isinstance(v, torch.Tensor) and v.dtype in (torch.float32, torch.bfloat16, torch.float16):
+                    v.copy_(torch.randn(v.shape, generator=gen) * 1e-3)
+    return opt
+
+
+def _same_state(a, b):
+    for group, other in zip(a.param_groups, b.param_groups):
+        for p, q in zip(group["params"], other["params"]):
+            assert set(a.state[p]) == set(b.state[q])
+            for k, v in a.state[p].items():
+                w = b.state[q][k]
+                if isinstance(v, torch.Tensor):
+                    assert w.dtype is v.dtype, k
+                    assert torch.equal(w.reshape(-1).view(torch.uint8), v.reshape(-1).view(torch.uint8)), k
+                else:
+                    assert w == v, k
+
+
+def _groups(**opts):
+    torch.manual_seed(0)
+    ps = [torch.nn.Parameter((torch.randn(s) * 0.02).bfloat16()) for s in ((6, 10), (40,))]
+    return [{"params": ps[:1], "lr": 1e-3, "orthogonalize": True, **opts},
+            {"params": ps[1:], "lr": 1e-3, "orthogonalize": False, **opts}]
+
+
+@pytest.mark.parametrize("opts", [dict(state_dtype=torch.float32), dict(state_dtype=torch.float32, decouple_md=True),
+                                  dict(state_dtype=torch.float16), dict(master_weights=True), dict(state_dtype=F8),
+                                  dict()])
+def test_saved_state_comes_back_in_its_types(opts):
+    """The base class casts floating state to the parameter's type; state that a group holds in
+    another one comes back as it was, bit for bit."""
+    opt = _with_state(_groups(**opts))
+    other = THORN(_groups(**opts))
+    other.load_state_dict(opt.state_dict())
+    _same_state(opt, other)

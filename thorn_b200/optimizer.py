@@ -500,16 +500,16 @@ class THORN(Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """``Optimizer.load_state_dict``, which casts state to the parameter's dtype, with the
-        8-bit codes and scales and the fp32 state beside master weights as they were saved."""
+        moments of groups that name a ``state_dtype``, the 8-bit codes and scales and the fp32
+        state beside master weights as they were saved."""
         super().load_state_dict(state_dict)
-        saved = [k for g in state_dict["param_groups"] for k in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for k, p in zip(saved, params):
-            old = state_dict["state"].get(k, {})
-            if "moment_scale" in old or "master" in old:
-                for key in ("moment", "variance", "moment_scale", "variance_scale", "master"):
-                    if key in old:
-                        self.state[p][key] = old[key].to(device=p.device)
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            for k, p in zip(saved["params"], group["params"]):
+                old = state_dict["state"].get(k, {})
+                if "moment_scale" in old or "master" in old or group.get("state_dtype") is not None:
+                    for key in ("moment", "variance", "moment_scale", "variance_scale", "master"):
+                        if key in old:
+                            self.state[p][key] = old[key].to(device=p.device)
 
     def _magma(self, items, cfg, recovered: bool, group=None) -> None:
         """Magma masking (thorn.py:806-836) for a list of launch records.
