@@ -60,3 +60,34 @@ def test_saved_state_comes_back_in_its_types(opts):
     other = THORN(_groups(**opts))
     other.load_state_dict(opt.state_dict())
     _same_state(opt, other)
+
+
+def test_load_hooks_decide_what_is_loaded():
+    """A hook that replaces the state dict before it is loaded is followed, and one that runs after
+    the load sees the state as it will be."""
+    opt = _with_state(_groups(state_dtype=F8, master_weights=True))
+    other = THORN(_groups(state_dtype=F8, master_weights=True))
+    seen = []
+
+    def zero_masters(optimizer, state_dict):
+        state = {k: {**v, "master": torch.zeros_like(v["master"])} for k, v in state_dict["state"].items()}
+        return {**state_dict, "state": state}
+
+    def after(optimizer):
+        for group in optimizer.param_groups:
+            for p in group["params"]:
+                st = optimizer.state[p]
+                seen.append((st["moment"].dtype, float(st["master"].abs().max())))
+                st["master"].fill_(2.0)
+
+    other.register_load_state_dict_pre_hook(zero_masters)
+    other.register_load_state_dict_post_hook(after)
+    other.load_state_dict(opt.state_dict())
+    assert seen == [(F8, 0.0)] * 2
+    for p, q in zip(*[[p for g in o.param_groups for p in g["params"]] for o in (opt, other)]):
+        assert bool((other.state[q]["master"] == 2).all()) and not bool((opt.state[p]["master"] == 2).any())
+        assert torch.equal(opt.state[p]["moment"].view(torch.uint8), other.state[q]["moment"].view(torch.uint8))
+    # nothing of the load stays behind: a second one runs the same two hooks
+    other.load_state_dict(opt.state_dict())
+    assert len(seen) == 4 and len(other._optimizer_load_state_dict_pre_hooks) == 1
+    assert len(other._optimizer_load_state_dict_post_hooks) == 1

@@ -51,6 +51,8 @@ from .coeffs import gram_ns_restarts, optimal_composition
 __all__ = ["THORN", "THORNOrthoGroup", "THORNNonOrthoGroup", "THORNGroup"]
 
 _TargetNorm = Union[Literal["init", "min", "max"], Callable[[torch.Tensor], Union[torch.Tensor, float]]]
+# state that load_state_dict keeps in the types it was saved in
+_KEPT_KEYS = ("moment", "variance", "moment_scale", "variance_scale", "master")
 LN_E_SUB_1 = 0.5413248546  # softplus(LN_E_SUB_1) == 1 (thorn.py:1602)
 
 # Magma momentum-aligned masking (thorn.py:806-836): score temperature and EMA
@@ -502,14 +504,34 @@ class THORN(Optimizer):
         """``Optimizer.load_state_dict``, which casts state to the parameter's dtype, with the
         moments of groups that name a ``state_dtype``, the 8-bit codes and scales and the fp32
         state beside master weights as they were saved."""
-        super().load_state_dict(state_dict)
-        for saved, group in zip(state_dict["param_groups"], self.param_groups):
-            for k, p in zip(saved["params"], group["params"]):
-                old = state_dict["state"].get(k, {})
-                if "moment_scale" in old or "master" in old or group.get("state_dtype") is not None:
-                    for key in ("moment", "variance", "moment_scale", "variance_scale", "master"):
-                        if key in old:
-                            self.state[p][key] = old[key].to(device=p.device)
+        kept = []  # for each group, for each parameter: what the base class must not cast
+
+        def take(_, saved):
+            state = dict(saved["state"])
+            for group in saved["param_groups"]:
+                kept.append([])
+                for k in group["params"]:
+                    old, own = state.get(k, {}), {}
+                    if "moment_scale" in old or "master" in old or group.get("state_dtype") is not None:
+                        own = {key: old[key] for key in _KEPT_KEYS if key in old}
+                        state[k] = {key: v for key, v in old.items() if key not in own}
+                    kept[-1].append(own)
+            return {**saved, "state": state}
+
+        def put(_):
+            for group, owns in zip(self.param_groups, kept):
+                for p, own in zip(group["params"], owns):
+                    for key, v in own.items():
+                        self.state[p][key] = v.to(device=p.device)
+
+        # behind the hooks that may replace the state dict, before those that look at what was loaded
+        before = self.register_load_state_dict_pre_hook(take)
+        after = self.register_load_state_dict_post_hook(put, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            before.remove()
+            after.remove()
 
     def _magma(self, items, cfg, recovered: bool, group=None) -> None:
         """Magma masking (thorn.py:806-836) for a list of launch records.
