@@ -91,3 +91,25 @@ def test_load_hooks_decide_what_is_loaded():
     other.load_state_dict(opt.state_dict())
     assert len(seen) == 4 and len(other._optimizer_load_state_dict_pre_hooks) == 1
     assert len(other._optimizer_load_state_dict_post_hooks) == 1
+
+
+def test_a_checkpoint_without_masters_says_so():
+    """torch takes a group's keys from the checkpoint: one that was saved without master weights
+    turns them off, and the load warns."""
+    import warnings
+
+    plain = _with_state(_groups())
+    other = THORN(_groups(master_weights=True))
+    with pytest.warns(UserWarning, match="without master weights"):
+        other.load_state_dict(plain.state_dict())
+    for opts in (dict(master_weights=True), dict()):  # nothing to say
+        opt, other = _with_state(_groups(**opts)), THORN(_groups(**opts))
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            other.load_state_dict(opt.state_dict())
+    fp32 = [torch.nn.Parameter(torch.zeros(4))]  # its own master
+    groups = [{"params": fp32, "lr": 1e-3, "orthogonalize": False}]
+    opt, other = THORN(groups), THORN([{**groups[0], "master_weights": True}])
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        other.load_state_dict(opt.state_dict())

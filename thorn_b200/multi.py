@@ -40,7 +40,7 @@ CODES = torch.float8_e4m3fn
 SCALES = torch.float8_e8m0fnu
 BLOCK = 128
 _U64 = (1 << 64) - 1
-_HALF = (torch.bfloat16, torch.float16)
+HALF = (torch.bfloat16, torch.float16)
 
 # layouts of thorn_adamw_state_tensor, thorn_momentum8_tensor and thorn_apply_master_tensor
 _ADAM = struct.Struct("<7QqQ3fi")
@@ -255,7 +255,7 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
     _pointers(rec, 0, size, params, pdt, dev, "params")
     _pointers(rec, 8, size, grads, pdt, dev, "grads", params, _SAME_SHAPE, distinct=False)
     if masters is not None:
-        if pdt not in _HALF:
+        if pdt not in HALF:
             raise TypeError(f"masters are fp32 copies of 16-bit parameters, got {pdt} parameters")
         _pointers(rec, 16, size, masters, torch.float32, dev, "masters", params, _SAME_SHAPE)
     _pointers(rec, 24, size, moments, sdt, dev, "moments", params, _SAME_SHAPE)
@@ -306,7 +306,7 @@ def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], sc
         return []
     dev, pdt = _device(grads[0]), grads[0].dtype
     N.dtype_code(pdt)
-    if dtype not in _HALF:
+    if dtype not in HALF:
         raise TypeError(f"the Newton-Schulz input is float16 or bfloat16, got {dtype}")
     if not 0.0 <= beta < 1.0:
         raise ValueError(f"beta must be in [0, 1), got {beta}")
@@ -343,7 +343,7 @@ def apply_update_(params: Sequence[torch.Tensor], updates: Sequence[torch.Tensor
     if n == 0:
         return
     dev, pdt, udt = _device(params[0]), params[0].dtype, updates[0].dtype
-    if pdt not in _HALF or udt not in _HALF:
+    if pdt not in HALF or udt not in HALF:
         raise TypeError(f"params and updates must be float16 or bfloat16, got {pdt} and {udt}")
     lrs = _per_tensor(lr, n, "lr")
     size = _APPLY.size

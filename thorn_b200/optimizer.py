@@ -33,6 +33,7 @@ Extensions (all optional, off by default):
 from __future__ import annotations
 
 import ctypes
+import warnings
 from dataclasses import MISSING, dataclass, field, fields
 from functools import partial
 from math import prod
@@ -415,7 +416,7 @@ class THORN(Optimizer):
 
     # ------------------------------------------------------------- routing
     def _init_state(self, p, state, cfg: GroupConfig, gdict):
-        master = bool(gdict.get("master_weights")) and p.dtype in (torch.bfloat16, torch.float16)
+        master = bool(gdict.get("master_weights")) and p.dtype in multi.HALF
         sdt = gdict.get("state_dtype") or (torch.float32 if master else p.dtype)
         eight = sdt is multi.CODES
         self._check_state_options(p, cfg, sdt, master)
@@ -503,7 +504,9 @@ class THORN(Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """``Optimizer.load_state_dict``, which casts state to the parameter's dtype, with the
         moments of groups that name a ``state_dtype``, the 8-bit codes and scales and the fp32
-        state beside master weights as they were saved."""
+        state beside master weights as they were saved.  The groups' keys are the saved ones, as
+        in the base class; a load that thereby turns master weights off warns."""
+        masters = [bool(group.get("master_weights")) for group in self.param_groups]
         kept = []  # for each group, for each parameter: what the base class must not cast
 
         def take(_, saved):
@@ -532,6 +535,10 @@ class THORN(Optimizer):
         finally:
             before.remove()
             after.remove()
+        for had, group in zip(masters, self.param_groups):
+            if had and not group.get("master_weights") and any(p.dtype in multi.HALF for p in group["params"]):
+                warnings.warn("the loaded state was saved without master weights: the group's 16-bit parameters go on "
+                              "being updated in place", stacklevel=2)
 
     def _magma(self, items, cfg, recovered: bool, group=None) -> None:
         """Magma masking (thorn.py:806-836) for a list of launch records.
