@@ -113,3 +113,41 @@ def test_a_checkpoint_without_masters_says_so():
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         other.load_state_dict(opt.state_dict())
+
+
+class _Cuda:
+    """torch.cuda's current device and capture state, for two devices of which the second captures."""
+
+    def __init__(self, monkeypatch):
+        self.now = 0
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: self.now)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.now == 1)
+        outer = self
+
+        class device:
+            def __init__(self, dev):
+                self.dev = torch.device(dev)
+
+            def __enter__(self):
+                self.old, outer.now = outer.now, self.dev.index
+
+            def __exit__(self, *exc):
+                outer.now = self.old
+
+        monkeypatch.setattr(torch.cuda, "device", device)
+
+
+def test_capture_is_looked_for_on_the_tensors_device(monkeypatch):
+    class T:
+        def __init__(self, dev):
+            self.device = torch.device(dev)
+
+    cuda = _Cuda(monkeypatch)
+    assert M._device(T("cuda:0")) == torch.device("cuda:0")
+    with pytest.raises(RuntimeError, match="captured"):
+        M._device(T("cuda:1"))
+    cuda.now = 1  # a capture on another device than the tensors'
+    assert M._device(T("cuda:0")) == torch.device("cuda:0")
+    with pytest.raises(RuntimeError, match="captured"):
+        M._device(T("cuda:1"))
+    assert cuda.now == 1

@@ -106,18 +106,23 @@ def _pointers(rec, offset, stride, ts, dtype, dev, what, like=None, mode=_ANY, d
     raise ValueError(f"{what}: the same tensor is given twice")
 
 
-def refuse_capture() -> None:
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("this call takes host scalars (step, learning rate, seeds) that a captured CUDA graph would "
-                           "repeat at every replay: call it outside of graph capture")
-
-
 _here = nullcontext()
 
 
 def _on(dev):
     """Makes ``dev`` the current device, which it mostly is already."""
     return _here if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def refuse_capture(dev) -> None:
+    """Raises where the current stream of ``dev`` is being captured."""
+    if dev.type != "cuda":
+        return
+    with _on(dev):
+        capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
+        raise RuntimeError("this call takes host scalars (step, learning rate, seeds) that a captured CUDA graph would "
+                           "repeat at every replay: call it outside of graph capture")
 
 
 def _stream(dev) -> int:
@@ -128,7 +133,7 @@ def _stream(dev) -> int:
 def _device(t) -> torch.device:
     if t.device.type != "cuda":
         raise RuntimeError(f"thorn_b200 runs its step on CUDA devices only; got a tensor on {t.device}")
-    refuse_capture()
+    refuse_capture(t.device)
     return t.device
 
 

@@ -670,8 +670,8 @@ class THORN(Optimizer):
             state = self.state[p]
             if "step" not in state:
                 self._init_state(p, state, cfg, gdict)
-            if ("moment_scale" in state or "master" in state) and _local(p).device.type == "cuda":
-                multi.refuse_capture()
+            if "moment_scale" in state or "master" in state:
+                multi.refuse_capture(_local(p).device)
             is_sharded = isinstance(p.data, DTensor) and not all(isinstance(pl, Replicate) for pl in p.placements)
             if is_sharded and cfg.orthogonalize:
                 sharded.append(p)
