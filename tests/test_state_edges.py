@@ -151,3 +151,26 @@ def test_capture_is_looked_for_on_the_tensors_device(monkeypatch):
     with pytest.raises(RuntimeError, match="captured"):
         M._device(T("cuda:1"))
     assert cuda.now == 1
+
+
+@pytest.mark.parametrize("opts", [dict(state_dtype=F8), dict(master_weights=True)])
+@pytest.mark.parametrize("ortho", [True, False])
+def test_a_refused_capture_leaves_no_state(monkeypatch, opts, ortho):
+    """State that is made during a capture would be filled by the graph's replays only."""
+    def capturing(dev):
+        raise RuntimeError("captured")
+
+    p = torch.nn.Parameter(torch.ones(8, 8, dtype=torch.bfloat16))
+    opt = THORN([{"params": [p], "lr": 1e-3, "orthogonalize": ortho, **opts}])
+    p.grad = torch.ones_like(p)
+    with monkeypatch.context() as m:
+        m.setattr(M, "refuse_capture", capturing)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()
+        assert "step" not in opt.state[p]
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        opt.step()
+    with monkeypatch.context() as m:  # state that is there: refused as well
+        m.setattr(M, "refuse_capture", capturing)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step()

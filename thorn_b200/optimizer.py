@@ -416,9 +416,8 @@ class THORN(Optimizer):
 
     # ------------------------------------------------------------- routing
     def _init_state(self, p, state, cfg: GroupConfig, gdict):
-        master = bool(gdict.get("master_weights")) and p.dtype in multi.HALF
+        eight, master = self._extended_state(p, state, gdict)
         sdt = gdict.get("state_dtype") or (torch.float32 if master else p.dtype)
-        eight = sdt is multi.CODES
         self._check_state_options(p, cfg, sdt, master)
         state["step"] = 1
         if eight:
@@ -468,6 +467,13 @@ class THORN(Optimizer):
                 seed = int(box[0])
             state["random_state"] = seed
             state["s"] = torch.ones((), dtype=p.dtype, device=_local(p).device)
+
+    @staticmethod
+    def _extended_state(p, state, gdict) -> tuple[bool, bool]:
+        """Whether p has, or gets at its first step, moments in 8 bits and a master copy."""
+        if "step" in state:
+            return "moment_scale" in state, "master" in state
+        return gdict.get("state_dtype") is multi.CODES, bool(gdict.get("master_weights")) and p.dtype in multi.HALF
 
     @staticmethod
     def _check_state_options(p, cfg: GroupConfig, sdt, master: bool) -> None:
@@ -668,10 +674,10 @@ class THORN(Optimizer):
                 if cfg.decouple_md or p.grad.sparse_dim() != 1:
                     p.grad = p.grad.to_dense()  # thorn.py:1667-1668
             state = self.state[p]
+            if any(self._extended_state(p, state, gdict)):
+                multi.refuse_capture(_local(p).device)  # before state is made whose filling would be captured
             if "step" not in state:
                 self._init_state(p, state, cfg, gdict)
-            if "moment_scale" in state or "master" in state:
-                multi.refuse_capture(_local(p).device)
             is_sharded = isinstance(p.data, DTensor) and not all(isinstance(pl, Replicate) for pl in p.placements)
             if is_sharded and cfg.orthogonalize:
                 sharded.append(p)
