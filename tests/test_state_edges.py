@@ -174,3 +174,25 @@ def test_a_refused_capture_leaves_no_state(monkeypatch, opts, ortho):
         m.setattr(M, "refuse_capture", capturing)
         with pytest.raises(RuntimeError, match="captured"):
             opt.step()
+
+
+def test_sparse_gradients_are_refused_by_the_state_that_is_there():
+    """A row update beside a master copy would be lost at the next dense step: the state decides,
+    also where the group's keys were changed after it was made; fp32 parameters of a group with
+    masters have none, and take sparse gradients as ever."""
+    def sparse(p):
+        return torch.sparse_coo_tensor(torch.tensor([[1]]), torch.ones(1, 8, dtype=p.dtype), (8, 8),
+                                       check_invariants=True)
+
+    for opts in (dict(state_dtype=F8), dict(master_weights=True)):
+        p = torch.nn.Parameter(torch.ones(8, 8, dtype=torch.bfloat16))
+        opt = _with_state([{"params": [p], "lr": 1e-3, "orthogonalize": False, **opts}])
+        opt.param_groups[0].update(state_dtype=None, master_weights=False)
+        p.grad = sparse(p)
+        with pytest.raises(NotImplementedError, match="sparse"):
+            opt.step()
+    p = torch.nn.Parameter(torch.ones(8, 8))
+    opt = THORN([{"params": [p], "lr": 1e-3, "orthogonalize": False, "master_weights": True}])
+    p.grad = sparse(p)
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        opt.step()

@@ -668,7 +668,7 @@ class THORN(Optimizer):
                 if cfg.orthogonalize or isinstance(p.data, DTensor):
                     raise NotImplementedError("sparse gradients are implemented for (R)AdamW parameters on one "
                                               "device only")
-                if gdict.get("state_dtype") is multi.CODES or gdict.get("master_weights"):
+                if any(self._extended_state(p, self.state.get(p, {}), gdict)):
                     raise NotImplementedError("sparse gradients with 8-bit state or master weights are not implemented "
                                               "by thorn_b200")
                 if cfg.decouple_md or p.grad.sparse_dim() != 1:
