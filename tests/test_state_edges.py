@@ -196,3 +196,46 @@ def test_sparse_gradients_are_refused_by_the_state_that_is_there():
     p.grad = sparse(p)
     with pytest.raises(RuntimeError, match="CUDA devices only"):
         opt.step()
+
+
+def _adam_args(ps):
+    return dict(params=ps, grads=[torch.zeros_like(p) for p in ps], moments=[torch.zeros_like(p) for p in ps],
+                variances=[torch.zeros_like(p) for p in ps], step=1, lr=1e-3)
+
+
+class _Launched(Exception):
+    pass
+
+
+@pytest.fixture
+def host_only(monkeypatch):
+    """The functions on CPU tensors up to the launch, which raises."""
+    def launch(*a, **k):
+        raise _Launched
+
+    monkeypatch.setattr(M, "_device", lambda t: t.device)
+    monkeypatch.setattr(M, "_on", lambda dev: M._here)
+    monkeypatch.setattr(M, "_stream", lambda dev: 0)
+    for name in ("launch_adam", "_momentum_call", "launch_apply"):
+        monkeypatch.setattr(M, name, launch)
+
+
+@pytest.mark.parametrize("order", [1, -1])
+def test_tensors_of_a_list_that_overlap_are_refused(host_only, order):
+    """Two entries of one list that share some of their memory would be written by two blocks at once."""
+    buf = torch.zeros(300, dtype=torch.bfloat16)
+    w = torch.zeros(300)
+    cuts = [((0, 100), (99, 200)), ((0, 300), (120, 130)), ((5, 6), (0, 300))]
+    touching = [((0, 100), (100, 200)), ((7, 9), (9, 10)), ((0, 0), (0, 300)), ((100, 100), (0, 300))]
+    for pairs, error in ((cuts, ValueError), (touching, _Launched)):
+        for pair in pairs:
+            ps, ws = [[t[a:b] for a, b in pair[::order]] for t in (buf, w)]
+            us = [p.half() for p in ps]
+            apart = [torch.zeros_like(p) for p in ps]
+            with pytest.raises(error):
+                M.apply_update_(ps, us, masters=[t.float() for t in apart], lr=1e-3)
+            with pytest.raises(error):
+                M.apply_update_(apart, us, masters=ws, lr=1e-3)
+            # what is only read may overlap
+            with pytest.raises(_Launched):
+                M.apply_update_(apart, ps, masters=[t.float() for t in apart], lr=1e-3)

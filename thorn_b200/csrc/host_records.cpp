@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <cstring>
 #include <exception>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -75,8 +76,8 @@ bool as_expected(const at::Tensor& t, const at::Tensor& like, int mode) {
 
 // pointers(records, offset, stride, tensors, dtype, device index or -1, like or None, mode,
 // distinct) -> bool: whether every tensor is a contiguous one of this dtype and device, of the
-// shape that `mode` derives from its partner in `like`, and (distinct) no two are the same
-// memory; their pointers are then in the records.
+// shape that `mode` derives from its partner in `like`, and (distinct) no two share memory;
+// their pointers are then in the records.
 PyObject* pointers(PyObject*, PyObject* args) {
   PyObject *buf, *list, *dtype, *like;
   Py_ssize_t offset, stride;
@@ -98,7 +99,7 @@ PyObject* pointers(PyObject*, PyObject* args) {
     if (!rec.ok) return nullptr;
     if (!rec.holds((Py_ssize_t)ts.size(), offset, stride, 8)) return bad_records();
     const at::ScalarType want = reinterpret_cast<THPDtype*>(dtype)->scalar_type;
-    std::vector<uint64_t> seen;
+    std::vector<std::pair<uint64_t, uint64_t>> seen;  // first byte, the one behind the last
     if (distinct) seen.reserve(ts.size());
     bool ascending = true;
     for (size_t i = 0; i < ts.size(); ++i) {
@@ -109,13 +110,14 @@ PyObject* pointers(PyObject*, PyObject* args) {
       const uint64_t p = (uint64_t)(uintptr_t)t.data_ptr();
       rec.put(i, offset, stride, p);
       if (distinct && numel_of(t) > 0) {  // empty tensors may share an address
-        ascending = ascending && (seen.empty() || seen.back() < p);
-        seen.push_back(p);
+        ascending = ascending && (seen.empty() || seen.back().second <= p);
+        seen.emplace_back(p, p + (uint64_t)numel_of(t) * t.element_size());
       }
     }
     if (!ascending) {
       std::sort(seen.begin(), seen.end());
-      if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_FALSE;
+      for (size_t i = 1; i < seen.size(); ++i)
+        if (seen[i].first < seen[i - 1].second) Py_RETURN_FALSE;
     }
   } catch (const std::exception& ex) {
     PyErr_SetString(PyExc_RuntimeError, ex.what());

@@ -103,7 +103,7 @@ def _pointers(rec, offset, stride, ts, dtype, dev, what, like=None, mode=_ANY, d
             raise ValueError(f"{what}[{i}] must be contiguous")
         if mode != _ANY and tuple(t.shape) != _expected_shape(like[i], mode):
             raise ValueError(f"{what}[{i}] must have shape {_expected_shape(like[i], mode)}, got {tuple(t.shape)}")
-    raise ValueError(f"{what}: the same tensor is given twice")
+    raise ValueError(f"{what}: the same tensor is given twice, or two share memory")
 
 
 _here = nullcontext()
