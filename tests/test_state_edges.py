@@ -239,3 +239,36 @@ def test_tensors_of_a_list_that_overlap_are_refused(host_only, order):
             # what is only read may overlap
             with pytest.raises(_Launched):
                 M.apply_update_(apart, ps, masters=[t.float() for t in apart], lr=1e-3)
+
+
+def test_writes_are_visible_to_autograd(host_only, monkeypatch):
+    """What a call writes counts as modified in place, as after torch's own operations: a graph that
+    saved it refuses to run backward.  What is only read, and refused calls, change nothing."""
+    for name in ("launch_adam", "_momentum_call", "launch_apply"):
+        monkeypatch.setattr(M, name, lambda *a, **k: None)
+    p = [torch.nn.Parameter(torch.ones(3, 50).bfloat16()) for _ in range(2)]
+    st = [M.state8_zeros(t) for t in p + p]
+    a = dict(params=p, grads=[torch.zeros_like(t) for t in p], moments=[c for c, _ in st[:2]],
+             variances=[c for c, _ in st[2:]], moment_scales=[s for _, s in st[:2]],
+             variance_scales=[s for _, s in st[2:]], masters=[t.detach().float() for t in p])
+    lists = [x for k, x in a.items() if k != "grads"]
+    loss = (p[0] * p[0]).sum()
+    was = [[t._version for t in x] for x in lists]
+    with pytest.raises(ValueError):
+        M.adamw_(**a, seeds=[1], step=1, lr=1e-3)
+    assert was == [[t._version for t in x] for x in lists]
+    M.adamw_(**a, seeds=[1, 2], step=1, lr=1e-3)
+    assert [[v + 1 for v in x] for x in was] == [[t._version for t in x] for x in lists]
+    assert all(g._version == 0 for g in a["grads"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    g, codes, scales = [torch.zeros(5, 7)], *[[t] for t in M.state8_zeros(torch.zeros(5, 7), per_matrix=True)]
+    out = [torch.zeros(5, 7, dtype=torch.float16)]
+    was = [t[0]._version for t in (codes, scales, out, g)]
+    M.momentum_(g, codes, scales, beta=0.9, seeds=[1], out=out)
+    assert [t[0]._version - v for t, v in zip((codes, scales, out, g), was)] == [1, 1, 1, 0]
+    q, w, u = [torch.zeros(4).bfloat16()], [torch.zeros(4)], [torch.zeros(4).half()]
+    M.apply_update_(q, u, masters=w, lr=1e-3)
+    assert (q[0]._version, w[0]._version, u[0]._version) == (1, 1, 0)
+    with torch.inference_mode():  # tensors without a version
+        M.apply_update_([torch.zeros(4).bfloat16()], [torch.zeros(4).half()], masters=[torch.zeros(4)], lr=1e-3)

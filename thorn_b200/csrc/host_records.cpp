@@ -278,6 +278,25 @@ PyObject* views(PyObject*, PyObject* args) {
   return out;
 }
 
+// written(list or None, ...): counts every tensor of the lists as modified in place, which a graph
+// that saved it looks at.  Inference tensors have no count.
+PyObject* written(PyObject*, PyObject* args) {
+  try {
+    for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(args); ++k) {
+      PyObject* list = PyTuple_GET_ITEM(args, k);
+      if (list == Py_None) continue;
+      std::vector<const at::Tensor*> ts;
+      if (!tensors_of(list, ts)) return nullptr;
+      for (const at::Tensor* t : ts)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    }
+  } catch (const std::exception& ex) {
+    PyErr_SetString(PyExc_RuntimeError, ex.what());
+    return nullptr;
+  }
+  Py_RETURN_NONE;
+}
+
 PyMethodDef kMethods[] = {
     {"pointers", pointers, METH_VARARGS, "check a list of tensors and write their pointers"},
     {"numels", numels, METH_VARARGS, "write element counts"},
@@ -285,6 +304,7 @@ PyMethodDef kMethods[] = {
     {"matrices", matrices, METH_VARARGS, "write batch, rows and columns"},
     {"scratch", scratch, METH_VARARGS, "write scratch pointers"},
     {"views", views, METH_VARARGS, "views of one buffer"},
+    {"written", written, METH_VARARGS, "count tensors as modified in place"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "thorn_b200_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

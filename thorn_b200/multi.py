@@ -18,9 +18,10 @@ gives one integer per tensor and should be new for every step (the same seeds gi
 
 ``THORN`` makes the same calls for groups with ``state_dtype=torch.float8_e4m3fn`` or
 ``master_weights=True``.  All functions run on the current stream of the tensors' device and
-change their tensors in place.  They take host scalars, which a captured CUDA graph would repeat at
-every replay, so they refuse to be captured.  The reference has no counterpart: it keeps state in
-the parameter's dtype (thorn.py:1591-1599) and updates 16-bit parameters in place.
+change their tensors in place, which autograd sees as it does torch's in-place operations.  They
+take host scalars, which a captured CUDA graph would repeat at every replay, so they refuse to be
+captured.  The reference has no counterpart: it keeps state in the parameter's dtype
+(thorn.py:1591-1599) and updates 16-bit parameters in place.
 """
 from __future__ import annotations
 
@@ -291,6 +292,7 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
             N.check(N.load().thorn_adamw_multi(N.array(N.AdamTensor, recs), n, N.dtype_code(pdt), N.dtype_code(sdt),
                                                float(b1), float(b2), float(weight_decay), float(eps), stream),
                     "adamw_multi")
+    host.written(params, moments, variances, ms, vs, masters)
 
 
 def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], scales: Sequence[torch.Tensor], *,
@@ -324,6 +326,7 @@ def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], sc
     _pointers(rec, 8, size, moments, CODES, dev, "moments", grads, _SAME_SHAPE)
     _pointers(rec, 16, size, scales, SCALES, dev, "scales", grads, _MATRIX_BLOCKS)
     host.values(rec, 64, size, n, "Q", seeds)
+    given = out
     if out is None:  # views of one allocation, each starting on 16 bytes
         out = host.views(torch.empty(elems, dtype=dtype, device=dev), grads, rec, 24, size)
     else:
@@ -332,6 +335,7 @@ def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], sc
     host.scratch(rec, 32, 72, size, n, _scratch_fn(), 0 if scratch is None else scratch.data_ptr())
     with _on(dev):
         _momentum_call(rec, pdt, dtype, float(beta), _stream(dev))
+    host.written(moments, scales, given)
     return out
 
 
@@ -363,6 +367,7 @@ def apply_update_(params: Sequence[torch.Tensor], updates: Sequence[torch.Tensor
     host.values(rec, 64, size, n, "f", lrs)
     with _on(dev):
         launch_apply(rec, udt, pdt, weight_decay, _stream(dev))
+    host.written(params, masters)
 
 
 # ------------------------------------------------------------------------------------ 8-bit state
