@@ -1,0 +1,71 @@
+"""Edges of the optimizer-state kernels on the GPU, against the definitions in float64 (state_reference.py).
+Error bounds as in test_state_gpu.py: an fp32 operation is off by at most 2^-24 of its result or,
+below the normal numbers, by 2^-150."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import state_reference as R
+import test_state_gpu as S
+
+pytestmark = pytest.mark.gpu
+
+E, TINY = 2.0 ** -24, 2.0 ** -150
+F8 = torch.float8_e4m3fn
+FORMS = ["8 bits", "8 bits and masters", "32 bits and masters"]
+
+
+def zero_state(n, form):
+    """Arguments of adamw_ for one tensor of n zeros with zero state; what it moves is in ["w"]."""
+    import thorn_b200 as T
+
+    p = [torch.zeros(n, device="cuda", dtype=torch.float32 if form == FORMS[0] else torch.bfloat16)]
+    a = dict(params=p, w=p[0])
+    if form != FORMS[0]:
+        a["masters"] = [torch.zeros(n, device="cuda")]
+        a["w"] = a["masters"][0]
+    if form == FORMS[2]:
+        a.update(moments=[torch.zeros(n, device="cuda")], variances=[torch.zeros(n, device="cuda")])
+    else:
+        (mc, ms), (vc, vs) = T.state8_zeros(p[0]), T.state8_zeros(p[0])
+        a.update(moments=[mc], variances=[vc], moment_scales=[ms], variance_scales=[vs], seeds=[3])
+    return a
+
+
+def step(a, g, **kw):
+    import thorn_b200 as T
+
+    args = {k: v for k, v in a.items() if k != "w"}
+    T.adamw_(**args, grads=[g.to(a["params"][0].dtype)], step=1, lr=1.0, **{"weight_decay": 0.0, **kw})
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("exponent", [-5, -12, -14, -15, -16, -17, -18, -19, -20, -22, -25, -32, -38])
+@pytest.mark.parametrize("spread", [0.0, 1.0])
+def test_small_gradients_keep_the_angle(form, exponent, spread):
+    """The first step from zero state is the angle of (g, |g|), pi / 4, at every magnitude whose
+    square fp32 holds, and towards pi / 2 as the square is lost: what float64 gives for the second
+    moment that fp32 holds.  ``spread``: neighbours over two more powers of ten."""
+    n = 1000
+    torch.manual_seed(1)
+    g = (torch.rand(n, device="cuda") + 0.5) * 10.0 ** exponent * 10.0 ** (2 * spread * (torch.rand(n, device="cuda") - 0.5))
+    g = g * (torch.randint(0, 2, (n,), device="cuda") * 2 - 1)
+    g[::50] = 0
+    a = zero_state(n, form)
+    g = g.to(a["params"][0].dtype)
+    step(a, g)
+    x, u = S.f64(g), -S.f64(a["w"])
+    # m: three operations on |g|; v: two products of numbers that may be below the normal ones
+    em = 5 * E * np.abs(x) + 3 * TINY
+    v, ev = 0.05 * x * x, 5 * E * 0.05 * x * x + 3 * TINY
+    bc1, bc2 = 1 / (1 - 0.9), 1 / (1 - 0.95)
+    hi = np.arctan2((0.1 * np.abs(x) + em) * bc1, np.sqrt(np.maximum(v - ev, 0) * bc2))
+    lo = np.arctan2(np.maximum(0.1 * np.abs(x) - em, 0) * bc1, np.sqrt((v + ev) * bc2))
+    some = x != 0
+    assert np.all(u[~some] == 0)
+    assert np.all(np.sign(u[some]) == np.sign(x[some]))
+    assert np.all(np.abs(u[some]) <= hi[some] * (1 + 16 * E)), np.abs(u[some]).max()
+    assert np.all(np.abs(u[some]) >= lo[some] * (1 - 16 * E)), np.abs(u[some]).min()

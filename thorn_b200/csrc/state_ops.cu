@@ -356,17 +356,51 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return r;
 }
 
-// atan2(y, sqrt(x2)) of two elements, x2 >= 0: with t = y / sqrt(x2), atan(s) for s = t where
-// |t| <= 1, else +-pi/2 + atan(s) for s = -1/t.  x2 is taken 2^-126 higher (nothing in fp32
-// from 2^-102 up), so that zero over zero is zero and a subnormal x2 needs no case of its
-// own; it acts like an eps of 1e-19 beside the root.  The polynomial in s^2 is the minimax
+// Second moments under 2^-94 (gradients near 1e-14 and smaller) are out of reach of the short
+// arithmetic below: zero over zero, and subnormal numbers, which the approximate instructions
+// flush.  A thread that finds one among its eight takes the scaled form for all of them.
+constexpr float kLowX2 = 5.0487097934144756e-29f;  // 2^-94
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ bool any_low(const f2* v) {
+  float x[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) unpack_f2(v[k], x[2 * k], x[2 * k + 1]);
+  return min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), fminf(x[6], x[7])) < kLowX2;
+}
+
+// The angle of y over the root of x2 is that of 2^110 y over the root of 2^220 x2: the smallest
+// x2 becomes 2^71 and the largest taken here 2^126.  A zero is taken as 2^-126: then zero over
+// zero is zero, and the smallest other y, 2^-39 after scaling, is 2^24 times its root.
+__device__ __forceinline__ void scale_low(float& y, float& x2) {
+  if (x2 < kLowX2) {
+    constexpr float s = 1.2980742146337069e33f;  // 2^110
+    y *= s;
+    x2 = fmaxf(x2 * s * s, 1.17549435e-38f);
+  }
+}
+__device__ __forceinline__ void scale_low2(f2& y, f2& x2) {
+  float y0, y1, q0, q1;
+  unpack_f2(y, y0, y1);
+  unpack_f2(x2, q0, q1);
+  scale_low(y0, q0);
+  scale_low(y1, q1);
+  y = pack_f2(y0, y1);
+  x2 = pack_f2(q0, q1);
+}
+
+// atan2(y, sqrt(x2)) of two elements, x2 a normal number: with t = y / sqrt(x2), atan(s) for
+// s = t where |t| <= 1, else +-pi/2 + atan(s) for s = -1/t.  The polynomial in s^2 is the minimax
 // fit of atan(s)/s on [0, 1] with eight coefficients (Remez exchange: 9.9e-8 relative,
 // 2.1e-7 with the roundings of its fp32 evaluation).  The general function, with an exact
 // square root and divisions, made the first 8-bit step of two 128256 x 4096 tensors 4108 us
 // where this made it 3103.
 __device__ __forceinline__ f2 angle2(f2 y, f2 x2) {
   float t0, t1, q0, q1;
-  unpack_f2(add(x2, dup(1.17549435e-38f)), q0, q1);
+  unpack_f2(x2, q0, q1);
   unpack_f2(mul(y, pack_f2(rsqrt_approx(q0), rsqrt_approx(q1))), t0, t1);
   float r0 = 0.f, r1 = 0.f;
   if (fabsf(t0) > 1.f) {
@@ -496,15 +530,21 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
   if (e.p == nullptr) return;
   if (!e.degenerate) {
     const f2 c = dup(e.c);
-    if (e.eps == 0.f) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) m[k] = angle2(mul(m[k], c), v[k]);
+    for (int k = 0; k < 4; ++k) m[k] = mul(m[k], c);
+    if (e.eps == 0.f) {
+      if (any_low(v)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) scale_low2(m[k], v[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m[k] = angle2(m[k], v[k]);
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float a, b;
         unpack_f2(v[k], a, b);
-        m[k] = mul(mul(m[k], c), pack_f2(rcp_approx(sqrt_approx(a) + e.eps), rcp_approx(sqrt_approx(b) + e.eps)));
+        m[k] = mul(m[k], pack_f2(rcp_approx(sqrt_approx(a) + e.eps), rcp_approx(sqrt_approx(b) + e.eps)));
       }
     }
   }
