@@ -376,8 +376,9 @@ THORN_API int thorn_magma_stats_multi(const thorn_magma_tensor* tensors, int n, 
  * 8-bit state: e4m3 codes, one byte per element, in blocks of 128 consecutive
  * elements with one scale byte each: value = code * 2^(byte - 127).  The byte is
  * the smallest with max|x| <= 448 * 2^(byte - 127) (at least 0; 0 for a block of
- * zeros).  A block that holds a value that is not finite gets byte 255 and reads
- * back as NaN.  Zeroed codes and scales are a zero state.  Codes are rounded
+ * zeros).  A block that holds a value that is not finite, or a finite one of
+ * 2^128 - 2^120 and more, gets byte 255 and reads back as NaN; values from
+ * 240 * 2^120 up may be rounded up to infinity.  Zeroed codes and scales are a zero state.  Codes are rounded
  * stochastically: |x| * 2^(127 - byte) rounds up with the probability of its
  * distance to the lower code, from 16 bits of a counter-based generator keyed by
  * `seed` (give every tensor and every step its own).  Elements 4q..4q+3 of a run
@@ -393,6 +394,9 @@ THORN_API int thorn_magma_stats_multi(const thorn_magma_tensor* tensors, int n, 
  *   update uses the moments before they are rounded.  In a block whose second
  *   moments are not all zero each is held at no less than the smallest code.
  * thorn_adamw_master_multi: fp32 moments and fp32 master weights.
+ * Both keep thorn_adamw_multi's formula at every magnitude, for the moments as
+ * fp32 holds them: an infinite gradient moves its parameter by lr times pi/4
+ * (NaN where eps > 0).
  * With w set (required by the second, optional for 16-bit parameters in the
  * first) the update is applied to w and p receives w rounded once.
  * ------------------------------------------------------------------------ */

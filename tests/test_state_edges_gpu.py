@@ -69,3 +69,23 @@ def test_small_gradients_keep_the_angle(form, exponent, spread):
     assert np.all(np.sign(u[some]) == np.sign(x[some]))
     assert np.all(np.abs(u[some]) <= hi[some] * (1 + 16 * E)), np.abs(u[some]).max()
     assert np.all(np.abs(u[some]) >= lo[some] * (1 - 16 * E)), np.abs(u[some]).min()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan, 1e30])
+@pytest.mark.parametrize("eps", [0.0, 1e-8])
+def test_infinite_gradients_move_like_the_definition(form, bad, eps):
+    """An infinite gradient has the angle of (inf, inf), pi / 4, as in the AdamW step on 16- and
+    32-bit state; over an eps it is inf / inf.  A finite one whose square is infinite moves nothing."""
+    a = zero_state(300, form)
+    g = torch.zeros(300, device="cuda")
+    g[130], g[7] = bad, 1e-3
+    step(a, g, eps=eps)
+    u = -S.f64(a["w"])
+    if math.isnan(bad) or (math.isinf(bad) and eps):
+        assert math.isnan(u[130])
+    else:
+        want = math.copysign(math.pi / 4, bad) if math.isinf(bad) else 0.0
+        assert abs(u[130] - want) <= 16 * E * abs(want)
+    rest = np.delete(u, [7, 130])
+    assert np.all(rest == 0) and np.isfinite(u[7]) and u[7] > 0

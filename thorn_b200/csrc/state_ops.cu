@@ -392,8 +392,25 @@ __device__ __forceinline__ void scale_low2(f2& y, f2& x2) {
   x2 = pack_f2(q0, q1);
 }
 
-// atan2(y, sqrt(x2)) of two elements, x2 a normal number: with t = y / sqrt(x2), atan(s) for
-// s = t where |t| <= 1, else +-pi/2 + atan(s) for s = -1/t.  The polynomial in s^2 is the minimax
+// Infinity over infinity is one over one.
+__device__ __forceinline__ void scale_infinite(float& y, float& x2) {
+  if (isinf(y) && isinf(x2)) {
+    y = copysignf(1.f, y);
+    x2 = 1.f;
+  }
+}
+__device__ __forceinline__ void scale_infinite2(f2& y, f2& x2) {
+  float y0, y1, q0, q1;
+  unpack_f2(y, y0, y1);
+  unpack_f2(x2, q0, q1);
+  scale_infinite(y0, q0);
+  scale_infinite(y1, q1);
+  y = pack_f2(y0, y1);
+  x2 = pack_f2(q0, q1);
+}
+
+// atan2(y, sqrt(x2)) of two elements, x2 a normal number, or infinite with y finite: with
+// t = y / sqrt(x2), atan(s) for s = t where |t| <= 1, else +-pi/2 + atan(s) for s = -1/t.  The polynomial in s^2 is the minimax
 // fit of atan(s)/s on [0, 1] with eight coefficients (Remez exchange: 9.9e-8 relative,
 // 2.1e-7 with the roundings of its fp32 evaluation).  The general function, with an exact
 // square root and divisions, made the first 8-bit step of two 128256 x 4096 tensors 4108 us
@@ -533,9 +550,13 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
 #pragma unroll
     for (int k = 0; k < 4; ++k) m[k] = mul(m[k], c);
     if (e.eps == 0.f) {
-      if (any_low(v)) {
+      // an 8-bit block with an infinite second moment has the scale byte 255
+      const bool infinite = S8 ? vb == 255u : top_up(v) >= 0x7f80ffffu;
+      if (any_low(v) || infinite) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) scale_low2(m[k], v[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) scale_infinite2(m[k], v[k]);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) m[k] = angle2(m[k], v[k]);
