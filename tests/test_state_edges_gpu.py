@@ -89,3 +89,27 @@ def test_infinite_gradients_move_like_the_definition(form, bad, eps):
         assert abs(u[130] - want) <= 16 * E * abs(want)
     rest = np.delete(u, [7, 130])
     assert np.all(rest == 0) and np.isfinite(u[7]) and u[7] > 0
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("eps", [1e-8, 1e-18, 1e-20, 1e-30, 1e-44, 1e-50])
+@pytest.mark.parametrize("exponent", [-10, -16, -19, -20, -25])
+def test_small_eps_beside_small_gradients(form, eps, exponent):
+    """g / (|g| + eps) in its float64 value for the moments that fp32 holds, also where the second
+    moment is below the normal numbers; an eps below them stays an eps."""
+    n = 400
+    torch.manual_seed(2)
+    g = (torch.rand(n, device="cuda") + 0.5) * 10.0 ** exponent
+    a = zero_state(n, form)
+    g = g.to(a["params"][0].dtype)
+    g[3] = 0
+    step(a, g, eps=eps)
+    x, u = S.f64(g), -S.f64(a["w"])
+    em = 5 * E * np.abs(x) + 3 * TINY
+    v, ev = 0.05 * x * x, 5 * E * 0.05 * x * x + 3 * TINY
+    low = max(eps, 2.0 ** -126)  # over a smaller one a zero second moment gives numbers near fp32's end
+    hi = (0.1 * x + em) * 10 / (np.sqrt(np.maximum(v - ev, 0) * 20) + min(eps, low))
+    lo = (0.1 * x - em) * 10 / (np.sqrt((v + ev) * 20) + low)
+    some = x != 0
+    assert np.all(u[~some] == 0)
+    assert np.all((u[some] <= hi[some] * (1 + 16 * E)) & (u[some] >= lo[some] * (1 - 16 * E)))

@@ -189,6 +189,7 @@ def adam_record(p, g, w, m, v, ms, vs, numel, seed, lr, bc1, bc2, degenerate) ->
 def launch_adam(records, p_dtype, eight: bool, betas, weight_decay: float, eps: float, stream) -> None:
     lib = N.load()
     fn = lib.thorn_adamw8_multi if eight else lib.thorn_adamw_master_multi
+    eps = max(eps, 2.0 ** -126) if eps > 0 else eps  # fp32 would round it to zero, which means the arc tangent
     N.check(fn(_records(N.AdamStateTensor, records), _count(_ADAM, records), N.dtype_code(p_dtype), float(betas[0]),
                float(betas[1]), float(weight_decay), float(eps), stream),
             "adamw8_multi" if eight else "adamw_master_multi")
