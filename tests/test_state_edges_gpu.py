@@ -113,3 +113,21 @@ def test_small_eps_beside_small_gradients(form, eps, exponent):
     some = x != 0
     assert np.all(u[~some] == 0)
     assert np.all((u[some] <= hi[some] * (1 + 16 * E)) & (u[some] >= lo[some] * (1 - 16 * E)))
+
+
+@pytest.mark.parametrize("form", FORMS[1:])
+def test_infinite_weights_without_decay_of_theirs(form):
+    """Where update and weight differ in sign nothing is decayed, whatever the weight is: an infinite
+    one stays infinite, as in the AdamW step on 16- and 32-bit state."""
+    import thorn_b200 as T
+
+    a = zero_state(40, form)
+    a["masters"][0][::2], a["masters"][0][1::2] = math.inf, -math.inf
+    a["params"][0].copy_(a["masters"][0])
+    g = torch.full((40,), -1e-3, device="cuda", dtype=torch.bfloat16)
+    g[1::2] *= -1
+    p, m, v = [a["params"][0].clone()], [torch.zeros(40, device="cuda")], [torch.zeros(40, device="cuda")]
+    T.adamw_(p, [g], m, v, step=1, lr=1.0, weight_decay=0.1)
+    step(a, g, weight_decay=0.1)
+    assert not bool(p[0].isnan().any())
+    assert torch.equal(a["params"][0], p[0]) and torch.equal(a["masters"][0], p[0].float())

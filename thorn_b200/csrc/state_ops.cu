@@ -590,11 +590,14 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
   f2 w[4];
   values(in.w, w);
   if (sc.wd > 0.f) {
+    const f2 wd = dup(sc.wd);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      float s0, s1;
+      float s0, s1, u0, u1, d0, d1;
       unpack_f2(mul(m[k], w[k]), s0, s1);
-      m[k] = fma(pack_f2(s0 >= 0.f ? sc.wd : 0.f, s1 >= 0.f ? sc.wd : 0.f), w[k], m[k]);
+      unpack_f2(m[k], u0, u1);
+      unpack_f2(fma(wd, w[k], m[k]), d0, d1);
+      m[k] = pack_f2(s0 >= 0.f ? d0 : u0, s1 >= 0.f ? d1 : u1);
     }
   }
   const f2 lr = dup(-e.lr);
