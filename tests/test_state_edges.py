@@ -272,3 +272,16 @@ def test_writes_are_visible_to_autograd(host_only, monkeypatch):
     assert (q[0]._version, w[0]._version, u[0]._version) == (1, 1, 0)
     with torch.inference_mode():  # tensors without a version
         M.apply_update_([torch.zeros(4).bfloat16()], [torch.zeros(4).half()], masters=[torch.zeros(4)], lr=1e-3)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_written_blocks_that_are_not_finite_hold_nan_codes(bad):
+    """As the kernels write them: they read a block's values as code times scale, and 255 is not a
+    scale that makes NaN of every code."""
+    x = torch.linspace(-1, 1, 300)
+    x[130] = bad
+    for positive in (False, True):
+        codes, scales = M.state8_write(x.abs() if positive else x, positive=positive)
+        c = codes.view(torch.uint8) & 127
+        assert bool((c[128:256] == 127).all()) and not bool((c[:128] == 127).any()) and not bool((c[256:] == 127).any())
+        assert scales.view(torch.uint8).tolist()[1] == 255

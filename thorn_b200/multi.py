@@ -415,6 +415,7 @@ def state8_write(x: torch.Tensor, per_matrix: bool = False, positive: bool = Fal
     byte = torch.where(torch.isfinite(top), byte, torch.full_like(byte, 255))
     scales.view(torch.uint8).copy_(byte.to(torch.uint8).reshape(scales.shape))
     y = torch.ldexp(v, (127 - byte.clamp_max(254))[..., None])
+    y = torch.where((byte < 255)[..., None], y, torch.full_like(y, float("nan")))
     if positive:
         y = torch.where((top > 0)[..., None], y.clamp_min(2.0 ** -9), y)
     y = y.reshape(runs, nb * BLOCK)[:, :n].clamp(-448, 448).to(CODES)
