@@ -378,7 +378,8 @@ THORN_API int thorn_magma_stats_multi(const thorn_magma_tensor* tensors, int n, 
  * the smallest with max|x| <= 448 * 2^(byte - 127) (at least 0; 0 for a block of
  * zeros).  A block that holds a value that is not finite, or a finite one of
  * 2^128 - 2^120 and more, gets byte 255 and reads back as NaN; values from
- * 240 * 2^120 up may be rounded up to infinity.  Zeroed codes and scales are a zero state.  Codes are rounded
+ * 240 * 2^120 up may be rounded up to infinity.  Zeroed codes and scales are a
+ * zero state.  Codes are rounded
  * stochastically: |x| * 2^(127 - byte) rounds up with the probability of its
  * distance to the lower code, from 16 bits of a counter-based generator keyed by
  * `seed` (give every tensor and every step its own).  Elements 4q..4q+3 of a run
@@ -420,6 +421,22 @@ THORN_API int thorn_adamw8_multi(const thorn_adamw_state_tensor* tensors, int n,
                                  double beta2, float weight_decay, float eps, void* stream);
 THORN_API int thorn_adamw_master_multi(const thorn_adamw_state_tensor* tensors, int n, int p_dtype, double beta1,
                                        double beta2, float weight_decay, float eps, void* stream);
+
+/* thorn_magma_stats_multi beside a moment in 8 bits: the sums of its values. */
+typedef struct {
+  const void* g;         /* as in thorn_magma_tensor */
+  const void* m;         /* e4m3 codes, same shape */
+  const void* m_scale;   /* scale bytes: ceil(run / 128) for each run of elements */
+  const void* row_gain;
+  const void* col_gain;
+  int64_t run;           /* rows * cols (blocks restart at each matrix) or batch * rows * cols */
+  int64_t batch, rows, cols;
+  double* out;
+  void* scratch;         /* as in thorn_magma_tensor */
+  int32_t scalar_gain;
+} thorn_magma8_tensor;
+
+THORN_API int thorn_magma_stats8_multi(const thorn_magma8_tensor* tensors, int n, int g_dtype, void* stream);
 
 /* Orthogonalized group with the momentum in 8 bits:  m <- beta1 m + g, rounded
  * to 8 bits (the blocks restart at each matrix of the batch);  u = g + beta1 m

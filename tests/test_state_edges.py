@@ -285,3 +285,36 @@ def test_written_blocks_that_are_not_finite_hold_nan_codes(bad):
         c = codes.view(torch.uint8) & 127
         assert bool((c[128:256] == 127).all()) and not bool((c[:128] == 127).any()) and not bool((c[256:] == 127).any())
         assert scales.view(torch.uint8).tolist()[1] == 255
+
+
+def test_magma8_record_and_refusals():
+    """Layout of the record, and bad arguments, which are refused before anything touches the device."""
+    import ctypes
+    import os
+    import subprocess
+    import tempfile
+
+    from thorn_b200 import _native as N
+
+    names = [f for f, _ in N.Magma8Tensor._fields_]
+    with tempfile.TemporaryDirectory() as d:
+        src = "".join(f'printf("%zu\\n", offsetof(thorn_magma8_tensor, {f}));' for f in names)
+        open(f"{d}/a.c", "w").write('#include <stdio.h>\n#include <stddef.h>\n#include "thorn_b200.h"\nint main(void) {'
+                                    + src + 'printf("%zu\\n", sizeof(thorn_magma8_tensor)); return 0; }')
+        subprocess.run(["gcc", "-I", B.INCLUDE, f"{d}/a.c", "-o", f"{d}/a"], check=True)
+        want = [int(x) for x in subprocess.run([f"{d}/a"], capture_output=True, text=True, check=True).stdout.split()]
+    assert want == [getattr(N.Magma8Tensor, f).offset for f in names] + [ctypes.sizeof(N.Magma8Tensor)]
+    lib, P = N.load(), 1 << 20
+
+    def call(n=1, dt=N.BF16, **kw):
+        t = N.Magma8Tensor(P, P, P, None, None, 60, 2, 6, 10, P, P, 0)
+        for k, v in kw.items():
+            setattr(t, k, v)
+        return lib.thorn_magma_stats8_multi(N.array(N.Magma8Tensor, [t]), n, dt, None)
+
+    assert call(n=0) == 0 and call(rows=0, run=0) == 0
+    assert call(n=-1) == 1 and call(dt=9) == 1 and call(batch=-1) == 1
+    for k in ("g", "m", "m_scale", "out", "scratch"):
+        assert call(**{k: None}) == 1, k
+    assert call(run=61) == 1 and call(run=0) == 1
+    assert call(row_gain=P) == 1  # split gains without the columns'

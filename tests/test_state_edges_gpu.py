@@ -131,3 +131,59 @@ def test_infinite_weights_without_decay_of_theirs(form):
     step(a, g, weight_decay=0.1)
     assert not bool(p[0].isnan().any())
     assert torch.equal(a["params"][0], p[0]) and torch.equal(a["masters"][0], p[0].float())
+
+
+@pytest.mark.parametrize("dtype", S.DTYPES)
+@pytest.mark.parametrize("per_matrix", [True, False])
+@pytest.mark.parametrize("gain", [None, "scalar", "split"])
+def test_magma_sums_of_8_bit_moments(dtype, per_matrix, gain):
+    """The three sums beside codes and scales are bit for bit those beside their fp32 values: whole
+    and ragged rows, blocks that end inside a row's eight, stacks, an unaligned copy, a NaN block."""
+    import types
+
+    import thorn_b200 as T
+    from thorn_b200.optimizer import GroupConfig
+
+    shapes = [(64, 256), (70, 300), (3, 5, 77), (2, 3, 9, 13), (1, 1), (200, 8), (4, 130, 131), (9, 40, 24)]
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    opt = T.THORN([{"orthogonalize": True, "params": [torch.nn.Parameter(torch.zeros(2, 2, device="cuda"))], "lr": 1e-3,
+                    "decouple_md": gain is not None}])
+    cfg = GroupConfig.from_kwargs(**opt.param_groups[0])
+    plain, eight = [], []
+    for i, s in enumerate(shapes):
+        g = (torch.randn(s, generator=gen, device="cuda") * 1e-3).to(dtype)
+        x = torch.randn(s, generator=gen, device="cuda") * 10.0 ** torch.randint(-6, 3, s[:-1] + (1,), generator=gen, device="cuda")
+        if i == 1:
+            x.view(-1)[500] = math.nan
+        codes, scales = T.state8_write(x, per_matrix=per_matrix)
+        if i % 2:
+            codes = S.offset_like(codes, 3)
+        gains = {}
+        if gain == "scalar":
+            gains = dict(gain=torch.rand((), generator=gen, device="cuda").to(dtype))
+        elif gain == "split":
+            gains = dict(row_gain=torch.rand(s[:-1] + (1,), generator=gen, device="cuda").to(dtype),
+                         col_gain=torch.rand(s[:-2] + (1, s[-1]), generator=gen, device="cuda").to(dtype))
+        for out, st in ((plain, dict(moment=T.state8_read(codes, scales))), (eight, dict(moment=codes, moment_scale=scales))):
+            out.append(types.SimpleNamespace(g=g, state={**st, **gains}, split=gain == "split"))
+    a, b = [opt._magma_stats(its, cfg, True).cpu() for its in (plain, eight)]
+    assert torch.equal(a.isnan(), b.isnan()) and bool(a[1].isnan().any()) and not bool(a[0].isnan().any())
+    assert torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+def test_magma_keeps_8_bit_moments_in_8_bits():
+    """Magma beside 8-bit state takes no copy of the moments: 64 Mi elements, well under a byte each."""
+    import thorn_b200 as T
+
+    p = torch.nn.Parameter(torch.zeros(8192, 8192, device="cuda", dtype=torch.bfloat16))
+    opt = T.THORN([{"orthogonalize": False, "params": [p], "lr": 1e-3, "momentum_align": True, "state_dtype": F8}])
+    p.grad = torch.full_like(p, 1e-3)
+    opt.step()
+    g = torch.full_like(p, 1e-3)
+    p.grad = g
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    opt.step()
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < p.numel() // 8

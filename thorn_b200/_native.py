@@ -79,6 +79,12 @@ class ApplyMasterTensor(Structure):
                 ("batch", c_int64), ("rows", c_int64), ("cols", c_int64), ("lr", c_float)]
 
 
+class Magma8Tensor(Structure):
+    _fields_ = [("g", c_void_p), ("m", c_void_p), ("m_scale", c_void_p), ("row_gain", c_void_p), ("col_gain", c_void_p),
+                ("run", c_int64), ("batch", c_int64), ("rows", c_int64), ("cols", c_int64), ("out", c_void_p),
+                ("scratch", c_void_p), ("scalar_gain", c_int32)]
+
+
 class MdPrepTensor(Structure):
     _fields_ = [("gain", c_void_p), ("sp", c_void_p), ("sig", c_void_p), ("n", c_int64)]
 
@@ -147,6 +153,7 @@ _STATE_PROTOS = {
                                    c_void_p]),
     "thorn_adamw_master_multi": (c_int, [POINTER(AdamStateTensor), c_int, c_int, c_double, c_double, c_float, c_float,
                                          c_void_p]),
+    "thorn_magma_stats8_multi": (c_int, [c_void_p, c_int, c_int, c_void_p]),  # Magma8Tensor records
     "thorn_momentum8_scratch_bytes": (c_int64, [c_int64, c_int64, c_int64]),
     "thorn_momentum8_multi": (c_int, [POINTER(Momentum8Tensor), c_int, c_int, c_int, c_float, c_void_p]),
     "thorn_apply_master_multi": (c_int, [POINTER(ApplyMasterTensor), c_int, c_int, c_int, c_float, c_void_p]),

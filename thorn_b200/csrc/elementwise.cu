@@ -871,9 +871,48 @@ __host__ __device__ inline int64_t magma_bytes(int64_t B, int64_t R, int64_t C) 
   return 16 + 3 * B * tiles_per_mat(R, C) * 8;
 }
 
+template <class E>
 struct MagmaArgs {
-  Pack<thorn_magma_tensor> pk;
+  Pack<E> pk;
 };
+
+// The moment's values at the elements off .. off + nc - 1 of a row of matrix b, zeros behind.
+template <class M>
+__device__ __forceinline__ void magma_moment(const thorn_magma_tensor& e, int64_t, int64_t off, int nc, bool vec,
+                                             float* m) {
+  load_n((const M*)e.m + off, m, nc, vec);
+}
+// From e4m3 codes and the power of two of each block of 128 (255: NaN); 8 elements lie in two
+// blocks at most.  Reading fp32 copies instead took 4 bytes per element of the whole group.
+template <class M>
+__device__ __forceinline__ void magma_moment(const thorn_magma8_tensor& e, int64_t b, int64_t off, int nc, bool vec,
+                                             float* m) {
+  const uint8_t* codes = (const uint8_t*)e.m + off;
+  uint32_t w[2] = {0u, 0u};
+  if (vec && nc == 8) {
+    const uint2 c = *reinterpret_cast<const uint2*>(codes);
+    w[0] = c.x;
+    w[1] = c.y;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < nc) w[k >> 2] |= (uint32_t)codes[k] << (8 * (k & 3));
+  }
+  const int64_t r = e.run == e.rows * e.cols ? b : 0, at = off - r * e.run;
+  const uint8_t* sp = (const uint8_t*)e.m_scale + r * ((e.run + 127) / 128);
+  const int64_t b0 = at >> 7, b1 = (at + nc - 1) >> 7;
+  auto scale = [](uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7fc00000u : max(byte << 23, 0x00400000u)); };
+  const float s0 = scale(sp[b0]), s1 = scale(sp[b1]);
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w[k >> 2] >> (8 * (k & 3)))));
+    float lo, hi;
+    unpack2(h, lo, hi, (__half*)nullptr);
+    m[k] = k < nc ? __fmul_rn(lo, ((at + k) >> 7) == b0 ? s0 : s1) : 0.f;
+    m[k + 1] = k + 1 < nc ? __fmul_rn(hi, ((at + k + 1) >> 7) == b0 ? s0 : s1) : 0.f;
+  }
+}
 
 // softplus(beta=1, threshold=20) rounded to the gain dtype, as F.softplus
 template <class G>
@@ -885,11 +924,11 @@ __device__ __forceinline__ float softplus_g(const G* gain, int64_t i) {
 // Each tile block sums g'*m, g'^2 and m^2 of its 64 x 256 tile (fp32 sums of eight
 // products, accumulated in fp64) and stores three partials; the last block of the
 // tensor adds all partials in tile order and writes the three fp64 totals.
-template <class G, class M>
-__global__ void __launch_bounds__(kThreads) magma_stats_kernel(const __grid_constant__ MagmaArgs a) {
+template <class G, class M, class E>
+__global__ void __launch_bounds__(kThreads) magma_stats_kernel(const __grid_constant__ MagmaArgs<E> a) {
   __shared__ double red[32];
   const int ti = find_tensor(a.pk, blockIdx.x);
-  const thorn_magma_tensor& e = a.pk.t[ti];
+  const E& e = a.pk.t[ti];
   const bool vec = a.pk.vec[ti];
   const int64_t lt = int64_t(blockIdx.x) - a.pk.start[ti];
   const Tile t = tile_of(lt, e.rows, e.cols);
@@ -917,7 +956,7 @@ __global__ void __launch_bounds__(kThreads) magma_stats_kernel(const __grid_cons
     const int64_t off = (t.b * e.rows + r) * e.cols + c;
     float g[8], m[8];
     load_n((const G*)e.g + off, g, nc, vec);
-    load_n((const M*)e.m + off, m, nc, vec);
+    magma_moment<M>(e, t.b, off, nc, vec, m);
     if (rg != nullptr) {
       if (e.scalar_gain) {
 #pragma unroll
@@ -1316,9 +1355,9 @@ extern "C" int64_t thorn_magma_scratch_bytes(int64_t batch, int64_t rows, int64_
   return magma_bytes(batch, rows, cols);
 }
 
-extern "C" int thorn_magma_stats_multi(const thorn_magma_tensor* ts, int n, int g_dtype, int m_dtype,
-                                       void* stream) {
-  if (n < 0 || (n > 0 && ts == nullptr) || !valid_dt(g_dtype) || !valid_dt(m_dtype)) return THORN_ERR_ARG;
+template <class E>
+static int magma_check(const E* ts, int n) {
+  if (n < 0 || (n > 0 && ts == nullptr)) return THORN_ERR_ARG;
   for (int i = 0; i < n; ++i) {
     const auto& e = ts[i];
     if (e.batch < 0 || e.rows < 0 || e.cols < 0) return THORN_ERR_ARG;
@@ -1326,18 +1365,41 @@ extern "C" int thorn_magma_stats_multi(const thorn_magma_tensor* ts, int n, int 
     if (!e.g || !e.m || !e.out || !e.scratch) return THORN_ERR_ARG;
     if (e.row_gain && !e.scalar_gain && !e.col_gain) return THORN_ERR_ARG;
   }
-  cudaStream_t st = (cudaStream_t)stream;
+  return THORN_OK;
+}
+template <class G, class M, class E>
+static int magma_launch(const E* ts, int n, int m_align, cudaStream_t st) {
+  auto blocks = [](const E& e) { return tiles_of(e.batch, e.rows, e.cols); };
+  auto vec = [m_align](const E& e) {
+    return (e.cols % 8) == 0 && aligned16(e.g) && (reinterpret_cast<uintptr_t>(e.m) & (m_align - 1)) == 0;
+  };
+  return launch_packed(ts, n, blocks, vec, [&](const Pack<E>& pk, int64_t nb) {
+    MagmaArgs<E> a;
+    a.pk = pk;
+    magma_stats_kernel<G, M, E><<<(unsigned)nb, kThreads, 0, st>>>(a);
+  });
+}
+
+extern "C" int thorn_magma_stats_multi(const thorn_magma_tensor* ts, int n, int g_dtype, int m_dtype,
+                                       void* stream) {
+  if (!valid_dt(g_dtype) || !valid_dt(m_dtype) || magma_check(ts, n)) return THORN_ERR_ARG;
   int rc = THORN_OK;
-  auto blocks = [](const thorn_magma_tensor& e) { return tiles_of(e.batch, e.rows, e.cols); };
-  auto vec = [](const thorn_magma_tensor& e) { return (e.cols % 8) == 0 && aligned16(e.g) && aligned16(e.m); };
   int d = dispatch2(g_dtype, m_dtype, [&](auto* pg, auto* pm) {
-    using G = std::remove_pointer_t<decltype(pg)>;
-    using M = std::remove_pointer_t<decltype(pm)>;
-    rc = launch_packed(ts, n, blocks, vec, [&](const Pack<thorn_magma_tensor>& pk, int64_t nb) {
-      MagmaArgs a;
-      a.pk = pk;
-      magma_stats_kernel<G, M><<<(unsigned)nb, kThreads, 0, st>>>(a);
-    });
+    rc = magma_launch<std::remove_pointer_t<decltype(pg)>, std::remove_pointer_t<decltype(pm)>>(
+        ts, n, 16, (cudaStream_t)stream);
+  });
+  return d ? d : rc;
+}
+
+extern "C" int thorn_magma_stats8_multi(const thorn_magma8_tensor* ts, int n, int g_dtype, void* stream) {
+  if (!valid_dt(g_dtype) || magma_check(ts, n)) return THORN_ERR_ARG;
+  for (int i = 0; i < n; ++i) {
+    const int64_t matrix = ts[i].rows * ts[i].cols, all = ts[i].batch * matrix;
+    if (all && (!ts[i].m_scale || (ts[i].run != matrix && ts[i].run != all))) return THORN_ERR_ARG;
+  }
+  int rc = THORN_OK;
+  int d = dispatch1(g_dtype, [&](auto* pg) {
+    rc = magma_launch<std::remove_pointer_t<decltype(pg)>, uint8_t>(ts, n, 8, (cudaStream_t)stream);
   });
   return d ? d : rc;
 }

@@ -565,9 +565,6 @@ class THORN(Optimizer):
             it.scale = 1.0
         if not cfg.momentum_align or not items:
             return
-        for it in items:
-            if "moment_scale" in it.state:
-                it.m_rows = multi.state8_read(it.state["moment"], it.state["moment_scale"])
         stats = self._magma_stats(items, cfg, recovered)
         scores = self._magma_scores(items, stats, group)
         for it, v in zip(items, scores):
@@ -609,15 +606,26 @@ class THORN(Optimizer):
         scr = self._scratch(dev, [lib.thorn_magma_scratch_bytes(B, R, C) for *_, B, R, C in recs])
         by_dt: dict = {}
         base = stats.data_ptr()
-        for i, ((g, m, rg, cg, scalar, B, R, C), sp) in enumerate(zip(recs, scr)):
+        eights: dict = {}
+        for i, (it, (g, m, rg, cg, scalar, B, R, C), sp) in enumerate(zip(items, recs, scr)):
             if rg is not None and rg.dtype != g.dtype:
                 raise TypeError("Magma: the gains must have the gradient dtype")
+            if m.dtype is multi.CODES:
+                scales = it.state["moment_scale"]
+                eights.setdefault(N.dtype_code(g.dtype), []).append(N.Magma8Tensor(
+                    g.data_ptr(), m.data_ptr(), scales.data_ptr(), None if rg is None else rg.data_ptr(),
+                    None if cg is None else cg.data_ptr(), R * C if scales.ndim == 2 else B * R * C, B, R, C,
+                    base + 24 * i, sp, scalar))
+                continue
             by_dt.setdefault((N.dtype_code(g.dtype), N.dtype_code(m.dtype)), []).append(N.MagmaTensor(
                 g.data_ptr(), m.data_ptr(), None if rg is None else rg.data_ptr(),
                 None if cg is None else cg.data_ptr(), scalar, B, R, C, base + 24 * i, sp))
         for (gc, mc), ts in by_dt.items():
             N.check(lib.thorn_magma_stats_multi(N.array(N.MagmaTensor, ts), len(ts), gc, mc, stream),
                     "magma_stats_multi")
+        for gc, ts in eights.items():
+            N.check(lib.thorn_magma_stats8_multi(N.array(N.Magma8Tensor, ts), len(ts), gc, stream),
+                    "magma_stats8_multi")
         del keep  # contiguous copies: freed in stream order after the launch
         return stats
 
@@ -639,8 +647,10 @@ class THORN(Optimizer):
             cdts = [torch.float32] * n
         else:
             cos = (stats[:, 0] / (stats[:, 1].sqrt().clamp_min(1e-8) * stats[:, 2].sqrt().clamp_min(1e-8))).float()
-            cdts = [torch.promote_types(it.g.dtype, (it.m_rows if getattr(it, "m_rows", None) is not None
-                                                     else _local(it.state["moment"])).dtype) for it in items]
+            mdts = [(it.m_rows if getattr(it, "m_rows", None) is not None else _local(it.state["moment"])).dtype
+                    for it in items]
+            cdts = [torch.promote_types(it.g.dtype, torch.float32 if mdt is multi.CODES else mdt)
+                    for it, mdt in zip(items, mdts)]
         keys: dict = {}
         for j, it in enumerate(items):
             keys.setdefault((cdts[j], it.state["s"].dtype), []).append(j)
