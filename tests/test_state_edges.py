@@ -318,3 +318,86 @@ def test_magma8_record_and_refusals():
         assert call(**{k: None}) == 1, k
     assert call(run=61) == 1 and call(run=0) == 1
     assert call(row_gain=P) == 1  # split gains without the columns'
+
+
+# ------------------------------------------------------------------ masters of sharded parameters
+def _sharded_masters(rank, world, port, q):
+    import datetime
+    import traceback
+
+    import torch.distributed as dist
+
+    try:
+        dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=world,
+                                timeout=datetime.timedelta(seconds=60))
+        from torch.distributed.device_mesh import init_device_mesh
+        from torch.distributed.tensor import DTensor, Shard, distribute_tensor
+
+        from thorn_b200 import _native as N
+        from thorn_b200.optimizer import GroupConfig
+
+        seen = []
+
+        class Lib:
+            def thorn_adamw_master_multi(self, recs, n, *scalars):
+                seen.extend((t.p, t.g, t.w, t.m, t.v, t.numel) for t in list(recs)[:n])
+                return 0
+
+        N.load = lambda build_if_missing=False: Lib()
+        N.stream_of = lambda dev: 0
+        mesh = init_device_mesh("cpu", (world,))
+        torch.manual_seed(0)
+        full = [torch.randn(s).bfloat16() for s in ((5, 3), (1,), (7,))]  # shards of different lengths, and an empty one
+
+        def make():
+            ps = [torch.nn.Parameter(distribute_tensor(t, mesh, [Shard(0)])) for t in full]
+            return ps, THORN([{"params": ps, "lr": 1e-3, "orthogonalize": False, "master_weights": True}])
+
+        ps, opt = make()
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+            opt._init_state(p, opt.state[p], GroupConfig.from_kwargs(**opt.param_groups[0]), opt.param_groups[0])
+            st = opt.state[p]
+            for k in ("master", "moment", "variance"):
+                assert isinstance(st[k], DTensor) and st[k].placements == p.placements
+                assert st[k].dtype is torch.float32 and st[k].to_local().shape == p.to_local().shape
+            assert torch.equal(st["master"].to_local(), p.to_local().float())
+        grads = [p.grad for p in ps]
+        opt._adam_local(ps, GroupConfig.from_kwargs(**opt.param_groups[0]))
+        loc = [[t.to_local() for t in (p.data, g, *[opt.state[p][k] for k in ("master", "moment", "variance")])]
+               for p, g in zip(ps, grads)]
+        assert [(*[x or 0 for x in r[:5]], r[5]) for r in seen] == \
+            [(*[t.data_ptr() for t in ts], ts[0].numel()) for ts in loc], (rank, seen)
+        opt.state[ps[0]]["master"].to_local().add_(1e-6)
+        qs, other = make()
+        other.load_state_dict(opt.state_dict())
+        for p, r in zip(ps, qs):
+            for k in ("master", "moment", "variance"):
+                a, b = opt.state[p][k], other.state[r][k]
+                assert b.dtype is a.dtype and b.placements == a.placements and torch.equal(a.to_local(), b.to_local())
+        dist.barrier()
+        dist.destroy_process_group()
+        q.put((rank, None))
+    except Exception:
+        q.put((rank, traceback.format_exc()))
+
+
+def test_masters_of_sharded_adamw_parameters():
+    """A Shard(0) parameter's master and moments are sharded alike, the step is given each rank's own
+    shards, and a load keeps them."""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_sharded_masters, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = [q.get(timeout=120) for _ in procs]
+    for p in procs:
+        p.join(60)
+    assert [err for _, err in got] == [None, None], got

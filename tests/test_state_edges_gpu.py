@@ -187,3 +187,256 @@ def test_magma_keeps_8_bit_moments_in_8_bits():
     opt.step()
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() - before < p.numel() // 8
+
+
+def decoded(codes, scales):
+    """float64 values of per-matrix state, [matrices, elements]."""
+    B = scales.shape[0]
+    return np.stack([R.read(c, s) for c, s in zip(S.u8(codes).reshape(B, -1), S.u8(scales).reshape(B, -1))])
+
+
+def test_more_matrices_than_a_launch_takes():
+    """70 short and long matrices and stacks: every pass of the momentum fills its table more than once."""
+    import thorn_b200 as T
+
+    kinds = [(3, 5), (40, 40), (65, 130), (2, 70, 90), (8, 16), (90, 100), (5, 64, 65)]
+    shapes = [kinds[i % 7] for i in range(70)]
+    g, m, s = S.make_matrices(shapes, torch.bfloat16, seed=7)
+    before = [decoded(c, r).reshape(-1) for c, r in zip(m, s)]
+    seeds = [11 * i for i in range(70)]
+    x = T.momentum_(g, m, s, beta=0.95, seeds=seeds)
+    torch.cuda.synchronize()
+    for i in range(70):
+        S.check_momentum(g[i], before[i], m[i], s[i], x[i], 0.95, seeds[i], torch.float16)
+
+
+def test_more_updates_than_a_launch_takes():
+    import thorn_b200 as T
+
+    torch.manual_seed(8)
+    shapes = [[(3, 5), (70, 130), (5000,)][i % 3] for i in range(70)]
+    w = [torch.randn(s, device="cuda") * 0.02 for s in shapes]
+    p = [t.bfloat16() for t in w]
+    u = [(torch.randn(s, device="cuda") * 0.05).half() for s in shapes]
+    lrs = [1e-2 * (1 + i % 5) for i in range(70)]
+    before = [S.f64(t) for t in w]
+    T.apply_update_(p, u, masters=w, lr=lrs, weight_decay=0.1)
+    for i in range(70):
+        uv = S.f64(u[i])
+        uv = np.where(uv * before[i] >= 0, uv + 0.1 * before[i], uv)
+        assert np.all(np.abs(S.f64(w[i]) - (before[i] - lrs[i] * uv)) <= 4 * E * (np.abs(before[i]) + lrs[i] * np.abs(uv)))
+        assert torch.equal(p[i], w[i].bfloat16())
+
+
+def test_stack_of_matrices_whose_norms_take_a_launch():
+    """Three matrices of 550 chunks each and of different magnitudes: each has its own norm."""
+    import thorn_b200 as T
+
+    g, m, s = S.make_matrices([(3, 1500, 1500)], torch.bfloat16, seed=9)
+    size = torch.tensor([1.0, 1e-3, 1e3], device="cuda").view(3, 1, 1)
+    g = [(g[0] * size).bfloat16()]
+    m, s = [[t] for t in T.state8_write(T.state8_read(m[0], s[0]) * size, per_matrix=True)]
+    before = decoded(m[0], s[0]).reshape(-1)
+    x = T.momentum_(g, m, s, beta=0.95, seeds=[12])
+    torch.cuda.synchronize()
+    S.check_momentum(g[0], before, m[0], s[0], x[0], 0.95, 12, torch.float16)
+
+
+def _big():
+    if torch.cuda.get_device_properties(0).total_memory < 120 << 30:
+        pytest.skip("needs 80 GB")
+
+
+@pytest.mark.parametrize("shape", [(65537, 65536), (3, 37901, 37901)])
+def test_momentum_offsets_beyond_32_bits(shape):
+    """More than 2^32 elements in one matrix and in a stack: the last 70000 elements, which start
+    inside a block, get the random numbers of their place; what lies before them stays zero."""
+    import thorn_b200 as T
+
+    _big()
+    tail = 70000
+    g = torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+    n, run = g.numel(), shape[-2] * shape[-1]
+    assert n > 1 << 32
+    torch.manual_seed(13)
+    g.view(-1)[n - tail:] = (torch.randn(tail, device="cuda") * 1e-3).bfloat16()
+    m, s = T.state8_zeros(g, per_matrix=True)
+    x, = T.momentum_([g], [m], [s], beta=0.95, seeds=[6])
+    last = run - tail
+    at = last // 128 * 128  # the block that the tail starts in, in its matrix
+    gv = S.f64(g.view(-1)[n - run + at:])
+    frac = R.fractions(run - at, 6, run=len(m.view(-1)) // run - 1, start=at)
+    new = R.check_state(gv, np.zeros(gv.size), S.u8(m.view(-1)[n - run + at:]), S.u8(s[-1, at // 128:]), frac, False, "m")
+    u = gv + 0.95 * new
+    norm = np.linalg.norm(u)
+    tol = (2.0 ** -11 + 2.0 ** 6 * E) * np.abs(u) / norm + 3 * E * (np.abs(gv) + np.abs(new)) / norm + 2.0 ** -25
+    assert np.all(np.abs(S.f64(x.view(-1)[n - run + at:]) - u / (norm + 1e-8)) <= tol)
+    head = (n - run + at) // 8 * 8
+    for t in (m.view(torch.uint8), x):
+        assert int(torch.count_nonzero(t.view(-1)[:head].view(torch.int64))) == 0
+
+
+def test_master_offsets_beyond_32_bits():
+    """AdamW and the apply onto fp32 masters of 2^32 + 5000 elements: the tail is updated, nothing before it."""
+    import thorn_b200 as T
+
+    _big()
+    n, tail = (1 << 32) + 5000, 4936
+    torch.manual_seed(14)
+    p, w = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, device="cuda")
+    g = torch.zeros(n, dtype=torch.float16, device="cuda")
+    g[n - tail:] = torch.randn(tail, device="cuda").half()
+    T.apply_update_([p], [g], masters=[w], lr=0.5, weight_decay=0.1)
+    assert torch.equal(w[n - tail:], -0.5 * g[n - tail:].float()) and torch.equal(p[n - tail:], w[n - tail:].bfloat16())
+    for t in (p, w):
+        assert int(torch.count_nonzero(t[:n - tail].view(torch.int64))) == 0
+    w[n - tail:] = 0
+    p[n - tail:] = 0
+    g = g.bfloat16()
+    m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    T.adamw_([p], [g], [m], [v], step=1, lr=1.0, weight_decay=0.0, masters=[w])
+    x = S.f64(g[n - tail:])
+    assert np.all(np.abs(S.f64(m[n - tail:]) - 0.1 * x) <= 5 * E * np.abs(x))
+    assert np.all(np.abs(S.f64(v[n - tail:]) - 0.05 * x * x) <= 5 * E * 0.05 * x * x)
+    want = -np.sign(x) * math.pi / 4
+    # pi / 4 is known to the errors of m and of the root of v: under 64 roundings
+    assert np.all(np.abs(S.f64(w[n - tail:]) - want) <= 64 * E)
+    for t in (p, w, m, v):
+        assert int(torch.count_nonzero(t[:n - tail].view(torch.int64))) == 0
+
+
+@pytest.mark.parametrize("ortho", [True, False])
+def test_decoupled_magnitudes_and_magma_beside_32_bit_state(ortho):
+    """Three steps of decouple_md and momentum_align, each beside one of fp32 state that holds the
+    same values: the same scores, masks and gains, moments that are the roundings of its, and for
+    AdamW, whose update uses the moments before they are rounded, the same parameters.  There the two
+    updates differ by at most 512 roundings of lr (32 of an angle up to pi / 2; 10 of |m| + |g| times
+    bc1 = 10 over a root of at least 0.9 |g|) and the passes behind them by 32 of the parameter."""
+    import thorn_b200 as T
+
+    shapes = [(64, 48), (40, 56), (3, 20, 30)]
+    p, q = [S._params(shapes, torch.float32, 6) for _ in range(2)]
+    opts = dict(orthogonalize=ortho, lr=1e-2, decouple_md=True, momentum_align=True, betas=(0.9, 0.95), none_grad=False)
+    a, b = T.THORN([{"params": p, "state_dtype": F8, **opts}]), T.THORN([{"params": q, **opts}])
+    grads = S._grads(p, 60)
+    moved = 0
+    for k in range(3):
+        if k:
+            for t, u in zip(p, q):
+                u.data.copy_(t.data)
+                for key, val in a.state[t].items():
+                    if key in ("moment", "variance"):
+                        b.state[u][key] = T.state8_read(val, a.state[t][key + "_scale"])
+                    elif "scale" not in key and key != "rounding_seed":
+                        b.state[u][key] = val.clone() if isinstance(val, torch.Tensor) else val
+        old = [{key: S.f64(b.state[u][key]) if k else np.zeros(u.numel()) for key in ("moment", "variance")} if
+               k == 0 or not ortho else {"moment": S.f64(b.state[u]["moment"])} for u in q]
+        at = [t.detach().clone() for t in p]
+        for opt, ps in ((a, p), (b, q)):
+            torch.manual_seed(70)
+            for t, x in zip(ps, grads):
+                t.grad = x.clone()
+            opt.step()
+        for i, (t, u) in enumerate(zip(p, q)):
+            s, w = a.state[t], b.state[u]
+            for key in w:
+                if key not in ("moment", "variance"):
+                    same = torch.equal(s[key], w[key]) if isinstance(w[key], torch.Tensor) else s[key] == w[key]
+                    assert same, (k, i, key)
+            B = int(np.prod(t.shape[:-2]))
+            g = S.f64(u.grad)  # the recovered gradient
+            assert torch.equal(t.grad, u.grad)
+            for key in ("moment", "variance") if not ortho else ("moment",):
+                err = 5 * E * (np.abs(old[i][key]) + np.abs(g)) if key == "moment" else 5 * E * S.f64(w[key])
+                runs = B if ortho else 1
+                cut = lambda z: z.reshape(runs, -1)  # noqa: E731
+                seed = (i << 32) + k + 1
+                for r in range(runs):
+                    R.check_state(cut(S.f64(w[key]))[r], cut(err)[r], cut(S.u8(s[key]))[r], cut(S.u8(s[key + "_scale"]))[r],
+                                  R.fractions(t.numel() // runs, seed, run=r), key == "variance", (k, i, key))
+            if not ortho:
+                assert bool(((t - u).abs() <= 512 * E * 1e-2 + 32 * E * u.abs()).all()), (k, i)
+            assert bool(t.isfinite().all())
+            moved += not torch.equal(t.detach(), at[i])
+    assert moved
+
+
+@pytest.mark.parametrize("ortho", [True, False])
+def test_a_refused_capture_leaves_the_steps_that_follow(ortho):
+    """A first step that was refused inside a capture, then two eager ones: what two steps give alone."""
+    import thorn_b200 as T
+
+    runs = []
+    for refused in (False, True):
+        p = S._params([(40, 48)], torch.bfloat16, 1)
+        opt = T.THORN([{"orthogonalize": ortho, "params": p, "lr": 1e-2, "state_dtype": F8, "master_weights": True}])
+        if refused:
+            p[0].grad = S._grads(p, 90)[0]
+            graph, x = torch.cuda.CUDAGraph(), torch.zeros(4, device="cuda")
+            with torch.cuda.graph(graph):
+                x.add_(1)
+                with pytest.raises(RuntimeError, match="capture"):
+                    opt.step()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert "step" not in opt.state[p[0]]
+        for k in range(2):
+            p[0].grad = S._grads(p, 90 + k)[0]
+            opt.step()
+        runs.append((p[0].detach(), opt.state[p[0]]["moment"].view(torch.uint8), opt.state[p[0]]["master"]))
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+
+
+def _one_rank(port, q):
+    import datetime
+    import traceback
+
+    import torch.distributed as dist
+
+    try:
+        torch.cuda.set_device(0)
+        dist.init_process_group("nccl", init_method=f"tcp://127.0.0.1:{port}", rank=0, world_size=1,
+                                timeout=datetime.timedelta(seconds=60), device_id=torch.device("cuda", 0))
+        from torch.distributed.device_mesh import init_device_mesh
+        from torch.distributed.tensor import Shard, distribute_tensor
+
+        import thorn_b200 as T
+
+        mesh = init_device_mesh("cuda", (1,))
+        plain = S._params([(50, 30), (7,)], torch.bfloat16, 1)
+        ps = [torch.nn.Parameter(distribute_tensor(t.detach().clone(), mesh, [Shard(0)])) for t in plain]
+        opts = dict(orthogonalize=False, lr=1e-2, master_weights=True, momentum_align=True)
+        a, b = T.THORN([{"params": plain, **opts}]), T.THORN([{"params": ps, **opts}])
+        for k in range(4):
+            for opt, group in ((a, plain), (b, ps)):
+                torch.manual_seed(30)
+                for t, x in zip(group, S._grads(plain, 10 + k)):
+                    t.grad = distribute_tensor(x, mesh, [Shard(0)]) if opt is b else x
+                opt.step()
+        for t, u in zip(plain, ps):
+            for x, y in ((t.detach(), u.data), *((a.state[t][k], b.state[u][k]) for k in ("master", "moment", "variance"))):
+                assert torch.equal(x, y.to_local())
+        torch.cuda.synchronize()
+        dist.destroy_process_group()
+        q.put(None)
+    except Exception:
+        q.put(traceback.format_exc())
+
+
+def test_masters_of_a_sharded_parameter_on_one_rank():
+    """A Shard(0) AdamW parameter of one rank steps like a plain one, Magma's sums over the shard group included."""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    p = ctx.Process(target=_one_rank, args=(port, q))
+    p.start()
+    err = q.get(timeout=180)
+    p.join(60)
+    assert err is None, err
