@@ -401,3 +401,52 @@ def test_masters_of_sharded_adamw_parameters():
     for p in procs:
         p.join(60)
     assert [err for _, err in got] == [None, None], got
+
+
+# ------------------------------------------------------------------------------------- the build
+def test_host_extension_is_of_this_torch_and_python(tmp_path, monkeypatch):
+    """Its file is named by what it is compiled against, so one of another torch or Python that
+    travelled with the tree is left alone."""
+    import sysconfig
+
+    from thorn_b200 import _native as N
+
+    assert torch.__version__ in B.HOST_LIB and sysconfig.get_config_var("SOABI") in B.HOST_LIB
+    assert N.host().__spec__.origin == B.HOST_LIB
+    monkeypatch.setattr(B, "LIB_DIR", str(tmp_path))
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    other = B.host_lib()
+    assert other != B.HOST_LIB and other.startswith(str(tmp_path))
+    (tmp_path / "given.so").write_bytes(open(B.HOST_LIB, "rb").read())
+    monkeypatch.setenv("THORN_B200_HOST_EXTENSION", str(tmp_path / "given.so"))
+    monkeypatch.setattr(N, "_host", None)
+    assert N.host().__spec__.origin == str(tmp_path / "given.so")
+    monkeypatch.setenv("THORN_B200_HOST_EXTENSION", str(tmp_path / "missing.so"))
+    monkeypatch.setattr(N, "_host", None)
+    with pytest.raises(RuntimeError, match="host extension not found"):
+        N.host()
+
+
+def test_the_library_is_built_without_the_host_extension(monkeypatch):
+    """A machine without a C++ compiler or torch's headers still gets the CUDA library, then the error."""
+    import subprocess
+
+    ran = []
+
+    def no_compiler(cmd, **kw):
+        ran.append(cmd[0])
+        raise FileNotFoundError(cmd[0])
+
+    monkeypatch.setattr(subprocess, "run", no_compiler)
+    monkeypatch.setattr(B, "_stale", lambda: False)
+    monkeypatch.setattr(B, "HOST_SRC", __file__)  # newer than the extension
+    monkeypatch.setattr(B.os.path, "getmtime", lambda p: float(p == __file__))
+    assert B.build_library() == B.LIB and not ran
+    with pytest.raises(FileNotFoundError):
+        B.build()
+    monkeypatch.setattr(B, "_stale", lambda: True)
+    monkeypatch.setattr(B, "_nvcc", lambda: "nvcc")
+    ran.clear()
+    with pytest.raises(FileNotFoundError):
+        B.build()
+    assert ran == ["nvcc"]  # the library comes first

@@ -177,7 +177,7 @@ def load(build_if_missing: bool = False):
         path = library_path()
         if not os.path.exists(path):
             if build_if_missing:
-                _build.build()
+                _build.build_library()
             else:
                 raise RuntimeError(
                     f"thorn_b200 CUDA library not found at {path}; build it with `python -m thorn_b200.build`")
@@ -199,10 +199,11 @@ def host():
     if _host is None:
         with _lock:
             if _host is None:
-                if not os.path.exists(_build.HOST_LIB):
-                    raise RuntimeError(f"thorn_b200 host extension not found at {_build.HOST_LIB}; build it with "
+                path = os.environ.get("THORN_B200_HOST_EXTENSION") or _build.HOST_LIB
+                if not os.path.exists(path):
+                    raise RuntimeError(f"thorn_b200 host extension not found at {path}; build it with "
                                        "`python -m thorn_b200.build`")
-                spec = importlib.util.spec_from_file_location("thorn_b200_host", _build.HOST_LIB)
+                spec = importlib.util.spec_from_file_location("thorn_b200_host", path)
                 module = importlib.util.module_from_spec(spec)
                 spec.loader.exec_module(module)
                 _host = module

@@ -1,8 +1,11 @@
 """Build the sm_100a shared library ``thorn_b200/_lib/libthorn_b200.so`` with nvcc, and the
-host extension ``thorn_b200/_lib/thorn_b200_host.so`` (``csrc/host_records.cpp``) with g++.
+host extension ``thorn_b200/_lib/thorn_b200_host.*.so`` (``csrc/host_records.cpp``) with g++.
 
 Usage: ``python -m thorn_b200.build [--force]``.  Both are built in-tree so they
-travel with the checkout; each is rebuilt when a source or header is newer.
+travel with the checkout; each is rebuilt when a source or header is newer.  The
+library, which is all that users of the C ABI need, comes first.  The extension's
+file is named by the torch and Python that it is compiled against: it reads
+libtorch's objects, and one of another version must not be loaded.
 """
 from __future__ import annotations
 
@@ -19,7 +22,6 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIB_DIR, "libthorn_b200.so")
-HOST_LIB = os.path.join(LIB_DIR, "thorn_b200_host.so")
 HOST_SRC = os.path.join(CSRC, "host_records.cpp")
 
 NVCC_FLAGS = [
@@ -49,6 +51,16 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def host_lib() -> str:
+    """The host extension's file for this torch and Python."""
+    import torch
+
+    return os.path.join(LIB_DIR, f"thorn_b200_host.torch-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so")
+
+
+HOST_LIB = host_lib()
+
+
 def build_host(force: bool = False, verbose: bool = False) -> str:
     """The CPython extension over this interpreter's libtorch."""
     if not force and os.path.exists(HOST_LIB) and os.path.getmtime(HOST_LIB) >= os.path.getmtime(HOST_SRC):
@@ -57,7 +69,7 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
 
     os.makedirs(LIB_DIR, exist_ok=True)
     root = os.path.dirname(torch.__file__)
-    tmp = HOST_LIB + ".tmp"
+    tmp = f"{HOST_LIB}.{os.getpid()}.tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            "-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
@@ -70,8 +82,8 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
     return HOST_LIB
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    build_host(force, verbose)
+def build_library(force: bool = False, verbose: bool = False) -> str:
+    """The CUDA library."""
     if not force and not _stale():
         return LIB
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -91,6 +103,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
     for o in objs:
         os.remove(o)
     return LIB
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    """Both; returns the library's path."""
+    lib = build_library(force, verbose)
+    build_host(force, verbose)
+    return lib
 
 
 if __name__ == "__main__":
