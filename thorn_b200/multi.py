@@ -18,8 +18,8 @@ gives one integer per tensor and should be new for every step (the same seeds gi
 
 ``THORN`` makes the same calls for groups with ``state_dtype=torch.float8_e4m3fn`` or
 ``master_weights=True``.  All functions run on the current stream of the tensors' device and
-change their tensors in place, which autograd sees as it does torch's in-place operations.  They
-take host scalars, which a captured CUDA graph would repeat at every replay, so they refuse to be
+change their tensors in place, which autograd sees as it does torch's in-place operations (not for
+8-bit state, which no operation saves).  They take host scalars, which a captured CUDA graph would repeat at every replay, so they refuse to be
 captured.  The reference has no counterpart: it keeps state in the parameter's dtype
 (thorn.py:1591-1599) and updates 16-bit parameters in place.
 """
@@ -47,6 +47,7 @@ HALF = (torch.bfloat16, torch.float16)
 _ADAM = struct.Struct("<7QqQ3fi")
 _MOMENTUM = struct.Struct("<4Q4qQQ")
 _APPLY = struct.Struct("<5Q3qf4x")
+_NO_POINTERS = (0,) * 7
 
 
 def _records(struct_type, parts):
@@ -112,15 +113,18 @@ _here = nullcontext()
 
 def _on(dev):
     """Makes ``dev`` the current device, which it mostly is already."""
-    return _here if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _here if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def refuse_capture(dev) -> None:
     """Raises where the current stream of ``dev`` is being captured."""
     if dev.type != "cuda":
         return
-    with _on(dev):
+    if torch._C._cuda_getDevice() == dev.index:  # the usual case, without a context
         capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(dev):
+            capturing = torch.cuda.is_current_stream_capturing()
     if capturing:
         raise RuntimeError("this call takes host scalars (step, learning rate, seeds) that a captured CUDA graph would "
                            "repeat at every replay: call it outside of graph capture")
@@ -132,10 +136,11 @@ def _stream(dev) -> int:
 
 
 def _device(t) -> torch.device:
-    if t.device.type != "cuda":
-        raise RuntimeError(f"thorn_b200 runs its step on CUDA devices only; got a tensor on {t.device}")
-    refuse_capture(t.device)
-    return t.device
+    dev = t.device
+    if dev.type != "cuda":
+        raise RuntimeError(f"thorn_b200 runs its step on CUDA devices only; got a tensor on {dev}")
+    refuse_capture(dev)
+    return dev
 
 
 @lru_cache(maxsize=4096)
@@ -258,7 +263,9 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
     if not eps >= 0.0:
         raise ValueError(f"eps must be >= 0, got {eps}")
     size = _ADAM.size
-    rec = bytearray(size * n)
+    scalars = _adam_scalars(steps, lrs, b1, b2, rectify, n)
+    one = not isinstance(scalars[0], list)  # the same four for all tensors
+    rec = bytearray(_ADAM.pack(*_NO_POINTERS, 0, 0, *scalars) * n if one else size * n)
     _pointers(rec, 0, size, params, pdt, dev, "params")
     _pointers(rec, 8, size, grads, pdt, dev, "grads", params, _SAME_SHAPE, distinct=False)
     if masters is not None:
@@ -281,8 +288,9 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
         if masters is not None and sdt is not torch.float32:
             raise TypeError(f"masters need fp32 or 8-bit moments, got {sdt}")
     host.numels(rec, 56, size, params)
-    for at, kind, column in zip((72, 76, 80, 84), "fffi", _adam_scalars(steps, lrs, b1, b2, rectify, n)):
-        host.values(rec, at, size, n, kind, column)
+    if not one:
+        for at, kind, column in zip((72, 76, 80, 84), "fffi", scalars):
+            host.values(rec, at, size, n, kind, column)
     with _on(dev):
         stream = _stream(dev)
         if eight or masters is not None:
@@ -293,7 +301,10 @@ def adamw_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
             N.check(N.load().thorn_adamw_multi(N.array(N.AdamTensor, recs), n, N.dtype_code(pdt), N.dtype_code(sdt),
                                                float(b1), float(b2), float(weight_decay), float(eps), stream),
                     "adamw_multi")
-    host.written(params, moments, variances, ms, vs, masters)
+    if eight:  # no operation saves codes or scales for a backward pass
+        host.written(params, masters)
+    else:
+        host.written(params, moments, variances, masters)
 
 
 def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], scales: Sequence[torch.Tensor], *,
@@ -336,7 +347,8 @@ def momentum_(grads: Sequence[torch.Tensor], moments: Sequence[torch.Tensor], sc
     host.scratch(rec, 32, 72, size, n, _scratch_fn(), 0 if scratch is None else scratch.data_ptr())
     with _on(dev):
         _momentum_call(rec, pdt, dtype, float(beta), _stream(dev))
-    host.written(moments, scales, given)
+    if given is not None:
+        host.written(given)
     return out
 
 
@@ -355,17 +367,17 @@ def apply_update_(params: Sequence[torch.Tensor], updates: Sequence[torch.Tensor
     dev, pdt, udt = _device(params[0]), params[0].dtype, updates[0].dtype
     if pdt not in HALF or udt not in HALF:
         raise TypeError(f"params and updates must be float16 or bfloat16, got {pdt} and {udt}")
-    lrs = _per_tensor(lr, n, "lr")
+    one = isinstance(lr, (int, float))
+    lrs = lr if one else _per_tensor(lr, n, "lr")
     size = _APPLY.size
-    rec = bytearray(size * n)
+    rec = bytearray(_APPLY.pack(*_NO_POINTERS[:5], 1, 1, 0, lrs if one else 0.0) * n)  # one row of all elements
     host = N.host()
     _pointers(rec, 8, size, params, pdt, dev, "params")
     _pointers(rec, 0, size, updates, udt, dev, "updates", params, _SAME_SHAPE, distinct=False)
     _pointers(rec, 16, size, masters, torch.float32, dev, "masters", params, _SAME_SHAPE)
-    host.values(rec, 40, size, n, "Q", 1)  # batch, rows: one row of all elements
-    host.values(rec, 48, size, n, "Q", 1)
     host.numels(rec, 56, size, params)
-    host.values(rec, 64, size, n, "f", lrs)
+    if not one:
+        host.values(rec, 64, size, n, "f", lrs)
     with _on(dev):
         launch_apply(rec, udt, pdt, weight_decay, _stream(dev))
     host.written(params, masters)
