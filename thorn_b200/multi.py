@@ -72,12 +72,12 @@ def _per_tensor(x, n: int, what: str) -> list:
 
 def _lists(**named):
     """The given tensor lists as lists of one length."""
-    out = {k: v if v is None or type(v) is list else list(v) for k, v in named.items()}
-    n = len(next(iter(out.values())))
-    for k, v in out.items():
+    out = [v if v is None or type(v) is list else list(v) for v in named.values()]
+    n = len(out[0])
+    for k, v in zip(named, out):
         if v is not None and len(v) != n:
             raise ValueError(f"{k}: {len(v)} tensors, expected {n}")
-    return list(out.values())
+    return out
 
 
 # what a list's tensors have to be like (host_records.cpp)
