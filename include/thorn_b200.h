@@ -397,7 +397,7 @@ THORN_API int thorn_magma_stats_multi(const thorn_magma_tensor* tensors, int n, 
  * thorn_adamw_master_multi: fp32 moments and fp32 master weights.
  * Both keep thorn_adamw_multi's formula at every magnitude, for the moments as
  * fp32 holds them: an infinite gradient moves its parameter by lr times pi/4
- * (NaN where eps > 0).
+ * (NaN where eps > 0).  An eps below the normal numbers counts as the smallest.
  * With w set (required by the second, optional for 16-bit parameters in the
  * first) the update is applied to w and p receives w rounded once.
  * ------------------------------------------------------------------------ */

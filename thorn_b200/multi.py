@@ -19,9 +19,9 @@ gives one integer per tensor and should be new for every step (the same seeds gi
 ``THORN`` makes the same calls for groups with ``state_dtype=torch.float8_e4m3fn`` or
 ``master_weights=True``.  All functions run on the current stream of the tensors' device and
 change their tensors in place, which autograd sees as it does torch's in-place operations (not for
-8-bit state, which no operation saves).  They take host scalars, which a captured CUDA graph would repeat at every replay, so they refuse to be
-captured.  The reference has no counterpart: it keeps state in the parameter's dtype
-(thorn.py:1591-1599) and updates 16-bit parameters in place.
+8-bit state, which no operation saves).  They take host scalars, which a captured CUDA graph would
+repeat at every replay, so they refuse to be captured.  The reference has no counterpart: it keeps
+state in the parameter's dtype (thorn.py:1591-1599) and updates 16-bit parameters in place.
 """
 from __future__ import annotations
 

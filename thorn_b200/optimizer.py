@@ -671,6 +671,7 @@ class THORN(Optimizer):
 
     def _step_params(self, params, cfg: GroupConfig, gdict):
         sharded, local = [], []
+        eager = set()  # devices whose current stream is known not to be captured
         for p in params:
             if p is None or p.grad is None:
                 continue
@@ -684,9 +685,13 @@ class THORN(Optimizer):
                 if cfg.decouple_md or p.grad.sparse_dim() != 1:
                     p.grad = p.grad.to_dense()  # thorn.py:1667-1668
             state = self.state[p]
-            if any(self._extended_state(p, state, gdict)):
-                multi.refuse_capture(_local(p).device)  # before state is made whose filling would be captured
-            if "step" not in state:
+            new = "step" not in state
+            if any(self._extended_state(p, state, gdict)) if new else ("moment_scale" in state or "master" in state):
+                dev = _local(p).device
+                if dev not in eager:  # before state is made whose filling would be captured
+                    multi.refuse_capture(dev)
+                    eager.add(dev)
+            if new:
                 self._init_state(p, state, cfg, gdict)
             is_sharded = isinstance(p.data, DTensor) and not all(isinstance(pl, Replicate) for pl in p.placements)
             if is_sharded and cfg.orthogonalize:
