@@ -440,3 +440,18 @@ def test_masters_of_a_sharded_parameter_on_one_rank():
     err = q.get(timeout=180)
     p.join(60)
     assert err is None, err
+
+
+def test_inputs_written_over_their_gradients():
+    """``out`` may be ``grads``: every length class, aligned and not, the same bits as apart."""
+    import thorn_b200 as T
+
+    shapes = [(5, 7, 9), (2, 64, 64), (9, 30, 30), (129, 127), (3, 65, 200), (1500, 1501)]
+    runs = []
+    for over in (False, True):
+        g, m, s = S.make_matrices(shapes, torch.float16, seed=15)
+        x = T.momentum_(g, m, s, beta=0.95, seeds=list(range(len(shapes))), out=g if over else None)
+        torch.cuda.synchronize()
+        runs.append([S.u8(t) for t in [*x, *m, *s]])
+    for a, b in zip(*runs):
+        assert np.array_equal(a, b)

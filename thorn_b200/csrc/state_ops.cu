@@ -611,13 +611,16 @@ __device__ __forceinline__ void adam_step8(const StAdam& e, const StAdamScalars&
 // and p receives their rounding.  EPS: the quotient, else the arc tangent (kernels of their own:
 // one with a branch on eps took 2.8 % longer for the two 128256 x 4096 tensors below).
 //
-// The 8-bit form of 16-bit parameters without masters is bound by instruction issue where the power cap holds the
-// clock down (two 128256 x 4096 tensors: 1.74 ms at 1.97 GHz, 1.85 at the 1.69 that a second of
-// it runs at), the others by DRAM.  It takes nine blocks per SM (56 registers): 1845 us
-// against 1869 at eight; without reading one turn ahead 1909 at eight and 1936 at twelve.
-// The forms that move more bytes per element take six (80 registers): 389 us for 151936 x
-// 1024 with masters, and 450 at the 86 registers that they take by themselves; the fp32 form
-// moves 28 bytes per element at the copy rate (659 us for that size).
+// The 8-bit form of 16-bit parameters without masters: 44 instructions per element.  Two
+// 128256 x 4096 tensors take 1690 us in a burst of 20 (0.97 of the copy rate) and 1955 where a
+// second of it has brought the clock down to 1.62 GHz at 1000 W: there instruction issue binds.
+// GPUs differ: 1890 to 2030 in other such runs.  On 16384 x 4096 (115 us) issue slots are 77 %
+// busy, DRAM 66 %, at 51 % of the warps.  Nine blocks per SM (56 registers): 1845 us against 1869
+// at eight, sustained, in one run of an earlier build; without reading one turn ahead 1909 at
+// eight and 1936 at twelve.
+// The others are bound by DRAM.  Those that move more bytes per element take six blocks (80
+// registers): 377 us for 151936 x 1024 with masters, 450 at the 86 registers that they once took by
+// themselves; the fp32 form moves 28 bytes per element at the copy rate (656 us for that size).
 template <class P, bool S8, bool MASTER, bool EPS, int CAP>
 __global__ void __launch_bounds__(kStThreads, S8 && !MASTER && sizeof(P) == 2 ? 9 : 6)
     adamw_state_kernel(const __grid_constant__ StAdamArgs<CAP> a) {
@@ -810,9 +813,11 @@ __device__ __forceinline__ float momentum_chunk(const StMomentum& e, float beta1
 }
 
 // The momentum pass: 4 bytes per element with 16-bit gradients, 19 instructions, which keep
-// the issue slots near 80 % busy at 89 % of the copy rate (153 us for the 218 M elements of a
-// decoder layer).  Twelve blocks per SM (40 registers): more loads in flight than at the
-// registers that it takes by itself (both passes 322 us against 339).
+// the issue slots 81 % busy (49 us for 16384 x 4096, its DRAM 61 %; both passes 312 us for the
+// 218 M elements of a decoder layer).  Twelve blocks per SM (40 registers): more loads in flight
+// than at the registers that it takes by itself (322 us against 339 in an earlier build).  The
+// bound is that of 16-bit gradients, which spill 8 bytes; fp32 ones spill 88 (14336 x 4096, both
+// passes: 136 us, 90 with bf16 gradients).
 template <class P, int CAP>
 __global__ void __launch_bounds__(kStThreads, 12) momentum8_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
   __shared__ float red[32];
@@ -884,7 +889,9 @@ __host__ __device__ inline int small_lanes(int64_t run) { return run <= 128 ? 16
 
 // One launch for all lengths: the 30 tensors of a small convolutional model took 15.2 us,
 // 19.5 with the lengths that need one turn in a launch of their own (five blocks per SM) and
-// 23.5 with a launch per form; 60000 matrices of 8 x 8 took 18.7 us against 16.5.
+// 23.5 with a launch per form; 60000 matrices of 8 x 8 took 18.7 us against 16.5 (floor 4.8: half
+// of the 16 lanes have nothing), and 4096 of 64 x 64 take 26.5 (floor 15.7).  The widest form's 80
+// registers, with 32 to 48 bytes of spills, are those of all three.
 template <class P, class X, int CAP>
 __global__ void __launch_bounds__(kStThreads, 6) momentum8_small_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
   __shared__ float red[32];
@@ -915,8 +922,10 @@ __global__ void __launch_bounds__(1024) momentum8_norm_kernel(const __grid_const
   if (threadIdx.x == 0) e.norm[b] = s;
 }
 
-// The input pass: 5 bytes per element, bound by DRAM (152 us for 218 M elements).  From the
-// last chunk to the first: what the momentum pass read and wrote last is then still in L2.
+// The input pass: 5 bytes per element, bound by DRAM (47 us for 16384 x 4096, DRAM 75 %).  From
+// the last chunk to the first: what the momentum pass read and wrote last is then still in L2.
+// Rows padded to a longer leading dimension take the element-wise stores: 4096 x 4097 into rows
+// of 4104 takes 74 us with its momentum pass, 31 in its own layout.
 template <class P, class X, int CAP>
 __global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __grid_constant__ StMomentumArgs<CAP> a) {
   __shared__ float red[32];
@@ -985,8 +994,10 @@ __global__ void __launch_bounds__(kStThreads) momentum8_input_kernel(const __gri
 // ===========================================================================
 // apply onto fp32 master weights
 // ===========================================================================
-// 12 bytes per element, bound by DRAM: 391 us for 218 M elements (6.7 TB/s); with the row and
-// matrix factors of a 14336 x 4096 matrix 116 us instead of 109.
+// 12 bytes per element, bound by DRAM: 391 us for 218 M elements (6.7 TB/s).  The factors are
+// formed for every 8 elements and again at each row that they cross: 14336 x 4096 takes 109 us
+// without, 111 with row factors and 116 with the matrix's as well; 4096 matrices of 40 x 39 take
+// 12.8, 16.8 and 32.4.
 struct StApply {
   const void* U;
   void* p;
@@ -1078,7 +1089,8 @@ __global__ void __launch_bounds__(kStThreads) apply_master_kernel(const __grid_c
 // Tensors per launch.  A launch costs more with a longer parameter: 4.8 us for one tensor at
 // a table of 32 (3 KB), 5.5 at 256.  The AdamW step, which meets many small tensors, takes a
 // table of 128 where it gets more than 32: 65 norm weights of 4096 took 21.2 us in three
-// launches of 32, 7.4 in one of 128, 11.3 in one of 256.
+// launches of 32, 7.4 in one of 128, 11.3 in one of 256.  Momentum and apply keep 32: 64 matrices
+// of 128 x 128 take 16.5 us, 32 of them 8.3.
 constexpr int kStCap = 32;
 constexpr int kStCapMany = 128;
 
